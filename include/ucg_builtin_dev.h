@@ -196,6 +196,8 @@ ucs_status_t ucg_builtin_dev_ctx_create(const ucg_builtin_dev_ctx_params_t *para
                                         ucg_builtin_dev_ctx_t **ctx_p);
 void         ucg_builtin_dev_ctx_destroy(ucg_builtin_dev_ctx_t *ctx);
 void        *ucg_builtin_dev_ctx_stream(ucg_builtin_dev_ctx_t *ctx);
+/* The HIP device ordinal of the context (-1 for NULL). */
+int          ucg_builtin_dev_ctx_device(const ucg_builtin_dev_ctx_t *ctx);
 /* Wait for all work queued on the context's stream(s). */
 ucs_status_t ucg_builtin_dev_sync(ucg_builtin_dev_ctx_t *ctx);
 /* Wait for the work queued on the context's launch stream the way the
@@ -257,6 +259,179 @@ ucs_status_t ucg_builtin_dev_reduce_tree(ucg_builtin_dev_ctx_t *ctx, ucg_dev_op_
                                          ucg_dev_dtype_t dt, void *dst,
                                          const void *const *srcs, unsigned nsrc,
                                          size_t count);
+
+/* ---- operators of a training step beside the combine ----------------------
+ *
+ * What a data-, tensor- or expert-parallel group computes around its combine:
+ * each result is either joined over the members with the combine above, or
+ * the same however the members cut the tensor. Like ucg_builtin_dev_reduce()
+ * they launch on the context's stream and return; every pointer but the
+ * params is device memory, aligned to its element. They allocate nothing and
+ * keep nothing between calls: a workspace is the caller's, 16-byte aligned,
+ * of at least the bytes its _workspace function names, and free for reuse by
+ * work that is ordered behind the call on the stream (calls that may run at
+ * once, or captured graphs that may replay at once, need one each). No
+ * reference counterpart (the reference combines, it does not train).
+ * FLOAT32, BFLOAT16 and FLOAT16 only; arithmetic in 32 bits or more, rounded
+ * once. Zero rows, columns or tokens are allowed unless stated otherwise. */
+
+/* dst = residual + dropout(sum of srcs + bias), rows x cols, contiguous.
+ *
+ * Element i (row-major) of the call is element g = offset + i of the whole
+ * tensor, and is kept if u(g) >= t, with t = p * 65536 rounded to the nearest
+ * integer (ties to even) and u(g) the 16 bits number g mod 8 of the 128 that
+ * Philox-4x32 with ten rounds (Salmon, Moraes, Dror, Shaw: Parallel random
+ * numbers: as easy as 1, 2, 3; SC 2011) gives for the counter (low, high word
+ * of g / 8, low, high word of tag) under the key (low, high word of seed),
+ * words in order, low half first. So the mask is never stored, and a shard of
+ * a tensor gets the whole tensor's mask there. Kept elements are multiplied
+ * by 65536 / (65536 - t): the mean is kept exactly, p itself to 2^-17.
+ * Dropped ones are exactly residual (0 without one), also where the sum is
+ * not finite. p = 1 drops everything, p = 0 draws nothing. */
+typedef struct ucg_builtin_dev_dropout_params {
+    int             dt;      /* ucg_dev_dtype_t of srcs, bias and dsrc */
+    int             out_dt;  /* ... of dst, residual and grad: dt or FLOAT32 */
+    size_t          rows;
+    size_t          cols;
+    double          p;       /* 0 <= p <= 1 */
+    uint64_t        seed;
+    uint64_t        tag;     /* one for each use under one seed (layer, step) */
+    uint64_t        offset;  /* place of the first element in the whole tensor */
+    const uint64_t *rng;     /* NULL, or device memory holding {seed, tag} to be
+                                used instead of those above (a captured graph
+                                replayed with other numbers) */
+} ucg_builtin_dev_dropout_params_t;
+
+/* The sum is of nsrc <= 16 sources in 32 bits, in the association of
+ * ucg_builtin_dev_reduce_multi() where nsrc is a power of two and of
+ * ucg_builtin_dev_reduce_tree() elsewhere; sources may be peer-mapped and may
+ * repeat. bias (cols elements) and residual may be NULL. dst may be the
+ * residual or, of the same type, any source; other overlap is refused. */
+ucs_status_t ucg_builtin_dev_sum_dropout(ucg_builtin_dev_ctx_t *ctx,
+                                         const ucg_builtin_dev_dropout_params_t *params,
+                                         void *dst, const void *const *srcs,
+                                         unsigned nsrc, const void *bias,
+                                         const void *residual);
+
+/* Its gradients: dsrc (of dt; every source's) = grad where kept, scaled, else
+ * 0; dbias (cols floats, or NULL) = the column sums of the same before dsrc is
+ * rounded, in a fixed order. The residual's gradient is grad itself. The
+ * params are the forward call's. dsrc may be grad where the types are equal.
+ * The workspace is needed only with dbias. */
+size_t       ucg_builtin_dev_sum_dropout_grad_workspace(size_t rows, size_t cols);
+ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
+                                              const ucg_builtin_dev_dropout_params_t *params,
+                                              void *dsrc, const void *grad, float *dbias,
+                                              void *workspace, size_t workspace_bytes);
+
+/* The balance loss of a router over `experts` experts (at most 1024), from
+ * its logits and the topk experts chosen for each token:
+ *
+ *   N = tokens that are not masked, c[e] = how often their indices name e,
+ *   P[e] = sum over them of softmax(logits)[e], z = sum of (log sum exp)^2
+ *   loss = balance_coef * experts / (topk * N^2) * sum c[e] P[e]
+ *        + z_coef / N * z
+ *
+ * The statistics add up over the members of a group: counts (INT64, experts +
+ * 1 values: c and N) and sums (FLOAT32, experts + 1 values: P and z) are what
+ * the group combines with SUM between _balance() and _balance_loss() /
+ * _balance_grad(). An index outside [0, experts) (a dropped choice) is
+ * counted nowhere. A logit of -inf has no probability; a row of them alone
+ * has none at all (no P, no z, gradient 0). Masked rows are not looked at:
+ * their gradient is 0 (base, where one is given). Without a token loss and
+ * gradients are 0. */
+typedef struct ucg_builtin_dev_balance_params {
+    int    dt;           /* ucg_dev_dtype_t of logits, dlogits and base */
+    int    index_dt;     /* UCG_DEV_DT_INT32 or UCG_DEV_DT_INT64 */
+    size_t tokens;
+    size_t experts;      /* 1 .. 1024 */
+    size_t topk;         /* 1 .. experts */
+    size_t ld;           /* elements from a row of logits to the next; 0 = experts */
+    size_t ld_index;     /* ... of index; 0 = topk */
+    size_t ld_out;       /* ... of dlogits and base; 0 = experts */
+    double balance_coef;
+    double z_coef;
+} ucg_builtin_dev_balance_params_t;
+
+/* counts and sums of this member's tokens; loss (3 floats: the loss, its
+ * balance and its z part; NULL = none) from these alone, for a group of one. */
+size_t       ucg_builtin_dev_balance_workspace(size_t tokens, size_t experts);
+ucs_status_t ucg_builtin_dev_balance(ucg_builtin_dev_ctx_t *ctx,
+                                     const ucg_builtin_dev_balance_params_t *params,
+                                     const void *logits, const void *index,
+                                     const uint8_t *mask, int64_t *counts, float *sums,
+                                     float *loss, void *workspace,
+                                     size_t workspace_bytes);
+/* loss (3 floats) from the group's counts and sums; uses experts, topk and
+ * the coefficients of params */
+ucs_status_t ucg_builtin_dev_balance_loss(ucg_builtin_dev_ctx_t *ctx,
+                                          const ucg_builtin_dev_balance_params_t *params,
+                                          const int64_t *counts, const float *sums,
+                                          float *loss);
+/* dlogits = base (0 where NULL) + grad_loss (1 where NULL) * dloss/dlogits,
+ * with the group's counts (which carry no gradient themselves). dlogits may be
+ * base or logits (of the same row step). */
+ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
+                                          const ucg_builtin_dev_balance_params_t *params,
+                                          const void *logits, const uint8_t *mask,
+                                          const int64_t *counts, const void *base,
+                                          const float *grad_loss, void *dlogits);
+
+/* The clipped policy loss with a KL term, over rows answers of up to cols
+ * tokens. For a token that is not masked, with A its advantage,
+ *
+ *   d = logp - old (rounded to 32 bits), r = exp(d), q = ref - logp
+ *   cut: A > 0 and d > log(1 + clip_high), or A < 0 and d < log(1 - clip_low)
+ *        (both limits rounded to 32 bits)
+ *   pg = -A * (cut ? 1 + clip_high or 1 - clip_low : r)
+ *   kl = exp(q) - q - 1 (0 without ref)
+ *   loss = mean of pg + kl_coef * mean of kl
+ *
+ * where the mean is over the group's tokens, or, with per_sequence, over the
+ * group's rows that have a token, of each row's mean. sums (FLOAT32, 2 values:
+ * the sums of pg and of kl, of the rows' means with per_sequence) and counts
+ * (INT64, 3 values: tokens, rows that have one, cut tokens) add up over the
+ * members of a group. Masked tokens are not looked at, whatever they hold:
+ * their gradient is 0. Without a token the loss is 0. */
+typedef struct ucg_builtin_dev_policy_params {
+    int    dt;            /* ucg_dev_dtype_t of logp, old, ref and dlogp */
+    int    adv_per_row;   /* adv holds rows values, else rows x cols */
+    int    per_sequence;
+    size_t rows;
+    size_t cols;
+    size_t ld;            /* elements from a row to the next of every rows x cols
+                             array; 0 = cols */
+    double clip_low;      /* 0 <= clip_low <= 1 */
+    double clip_high;     /* 0 <= clip_high */
+    double kl_coef;
+} ucg_builtin_dev_policy_params_t;
+
+/* adv is FLOAT32. ref and mask may be NULL. row_tokens (int32, rows values:
+ * each row's tokens; NULL = not wanted) is what _policy_grad() needs with
+ * per_sequence. loss: 3 floats (the loss, its pg and its kl mean), or NULL. */
+size_t       ucg_builtin_dev_policy_workspace(size_t rows, size_t cols);
+ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
+                                    const ucg_builtin_dev_policy_params_t *params,
+                                    const void *logp, const void *old, const void *ref,
+                                    const float *adv, const uint8_t *mask, float *sums,
+                                    int64_t *counts, int32_t *row_tokens, float *loss,
+                                    void *workspace, size_t workspace_bytes);
+/* loss (3 floats) from the group's sums and counts; uses per_sequence and
+ * kl_coef of params */
+ucs_status_t ucg_builtin_dev_policy_loss(ucg_builtin_dev_ctx_t *ctx,
+                                         const ucg_builtin_dev_policy_params_t *params,
+                                         const float *sums, const int64_t *counts,
+                                         float *loss);
+/* dlogp = grad_loss (1 where NULL) * dloss/dlogp, with the group's counts and,
+ * with per_sequence, this member's row_tokens. At a limit a token is not cut.
+ * dlogp may be logp, old or ref. */
+ucs_status_t ucg_builtin_dev_policy_grad(ucg_builtin_dev_ctx_t *ctx,
+                                         const ucg_builtin_dev_policy_params_t *params,
+                                         const void *logp, const void *old,
+                                         const void *ref, const float *adv,
+                                         const uint8_t *mask, const int32_t *row_tokens,
+                                         const int64_t *counts, const float *grad_loss,
+                                         void *dlogp);
 
 /* ---- host-resident combine (the reduce_cb_f contract, staged) ------------*/
 /* Whole-buffer: dst_host[i] = src_host[i] (op) dst_host[i]. Host chunks are

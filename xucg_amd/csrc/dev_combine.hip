@@ -270,6 +270,12 @@ int dev_ctx_device(const ucg_builtin_dev_ctx_t *ctx)
     return ctx->device;
 }
 
+void dev_ctx_count(ucg_builtin_dev_ctx_t *ctx, uint64_t launches, uint64_t bytes)
+{
+    ctx->counters[0] += launches;
+    ctx->counters[1] += bytes;
+}
+
 static ucs_status_t ring_init(ucg_builtin_dev_ctx_t *ctx)
 {
     if (ctx->h_ring) {
@@ -631,6 +637,11 @@ static ucs_status_t d2h_stream(ucg_builtin_dev_ctx_t *ctx)
 void *ucg_builtin_dev_ctx_stream(ucg_builtin_dev_ctx_t *ctx)
 {
     return ctx ? (void*)ctx->stream : nullptr;
+}
+
+int ucg_builtin_dev_ctx_device(const ucg_builtin_dev_ctx_t *ctx)
+{
+    return ctx ? ctx->device : -1;
 }
 
 ucs_status_t ucg_builtin_dev_sync(ucg_builtin_dev_ctx_t *ctx)

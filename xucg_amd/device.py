@@ -34,6 +34,26 @@ def _ptr(x):
     raise TypeError(f"cannot take a device pointer of {type(x)}")
 
 
+_DT = {name: i for i, name in enumerate(_lib.DTYPES)}
+
+
+class _TorchNames(dict):
+    """torch dtype -> its name here; filled on first sight, torch not imported"""
+    def __missing__(self, dtype):
+        name = self[dtype] = str(dtype).rpartition(".")[2]
+        return name
+
+    def get(self, dtype, default=None):
+        return self[dtype]
+
+
+_TORCH_NAME = _TorchNames()
+
+
+def _name(dt):
+    return dt if isinstance(dt, str) else _lib.DTYPES[dt]
+
+
 def dtype_size(dt):
     return DTYPE_SIZE[dt_index(dt)]
 
@@ -137,6 +157,7 @@ class DevContext:
         check(L.ucg_builtin_dev_ctx_create(ctypes.byref(p), ctypes.byref(h)),
               "ucg_builtin_dev_ctx_create")
         self.handle = h.value
+        self.device = L.ucg_builtin_dev_ctx_device(h)
 
     @classmethod
     def on_torch_stream(cls, device=0, **kw):
@@ -228,6 +249,200 @@ class DevContext:
         da = (ctypes.c_void_p * n)(*[_ptr(d) for d in dsts])
         sa = (ctypes.c_void_p * n)(*[_ptr(s) for s in srcs])
         return _lib.dev().ucg_builtin_dev_copy_multi(self.handle, da, sa, n, nbytes)
+
+    # -- operators of a training step beside the combine -------------------
+    def _operands(self, *specs):
+        """Addresses of (name, buffer, dtype, shape, row step) operands. A torch
+        tensor is held to them: the type, this context's device, as many
+        elements, and rows `row step` apart whose elements are neighbours."""
+        out = []
+        for name, x, dt, shape, ld in specs:
+            if x is None or isinstance(x, int) or not hasattr(x, "data_ptr"):
+                out.append(_ptr(x))
+                continue
+            if _TORCH_NAME.get(x.dtype) != dt and not (
+                    dt == "uint8" and _TORCH_NAME.get(x.dtype) == "bool"):
+                raise ValueError(f"{name}: {dt} wanted, got {x.dtype}")
+            if x.device.type != "cuda" or x.device.index != self.device:
+                raise ValueError(f"{name}: a tensor on cuda:{self.device} wanted, got one on "
+                                 f"{x.device}")
+            want = 1
+            for n in shape:
+                want *= n
+            if x.numel() < want if ld is None else x.numel() != want:
+                raise ValueError(f"{name}: {tuple(shape)} wanted, got {tuple(x.shape)}")
+            if not x.is_contiguous() or (ld or shape[-1]) != shape[-1]:
+                if not (ld and want and x.dim() == 2 and tuple(x.shape) == tuple(shape) and
+                        (shape[1] == 1 or x.stride(1) == 1) and
+                        (shape[0] == 1 or x.stride(0) == ld)):
+                    raise ValueError(f"{name}: strides {x.stride()} where rows of neighbours, "
+                                     f"{ld or shape[-1]} apart, are wanted")
+            out.append(x.data_ptr())
+        return out
+
+    def sum_dropout(self, dt, dst, srcs, rows, cols, p, seed, tag=0, offset=0, bias=None,
+                    residual=None, out_dt=None, rng=None):
+        """dst = residual + dropout(sum of srcs + bias), the mask a function of
+        (seed, tag, offset + element) that is never stored
+        (ucg_builtin_dev_sum_dropout)."""
+        dt, out_dt, shape = _name(dt), _name(dt if out_dt is None else out_dt), (rows, cols)
+        dst, bias, residual, rng, *srcs = self._operands(
+            ("dst", dst, out_dt, shape, cols), ("bias", bias, dt, (cols,), cols),
+            ("residual", residual, out_dt, shape, cols), ("rng", rng, "int64", (2,), 2),
+            *(("srcs", s, dt, shape, cols) for s in srcs))
+        q = _lib.DropoutParams(_DT[dt], _DT[out_dt], rows, cols, p, seed, tag, offset, rng)
+        check(_lib.dev().ucg_builtin_dev_sum_dropout(
+            self.handle, q, dst, (ctypes.c_void_p * len(srcs))(*srcs), len(srcs), bias,
+            residual), "ucg_builtin_dev_sum_dropout")
+
+    @staticmethod
+    def sum_dropout_grad_workspace(rows, cols):
+        """bytes of sum_dropout_grad's workspace (with dbias)"""
+        return _lib.dev().ucg_builtin_dev_sum_dropout_grad_workspace(rows, cols)
+
+    def sum_dropout_grad(self, dt, dsrc, grad, rows, cols, p, seed, tag=0, offset=0, dbias=None,
+                         grad_dt=None, workspace=None, rng=None):
+        """dsrc = the gradient of every source of sum_dropout, dbias (cols
+        floats) = the bias' (ucg_builtin_dev_sum_dropout_grad)."""
+        dt, grad_dt, shape = _name(dt), _name(dt if grad_dt is None else grad_dt), (rows, cols)
+        dsrc, grad, dbias, rng = self._operands(
+            ("dsrc", dsrc, dt, shape, cols), ("grad", grad, grad_dt, shape, cols),
+            ("dbias", dbias, "float32", (cols,), cols), ("rng", rng, "int64", (2,), 2))
+        q = _lib.DropoutParams(_DT[dt], _DT[grad_dt], rows, cols, p, seed, tag, offset, rng)
+        ws, nbytes = self._workspace(workspace, self.sum_dropout_grad_workspace, rows, cols)
+        check(_lib.dev().ucg_builtin_dev_sum_dropout_grad(self.handle, q, dsrc, grad, dbias, ws,
+                                                          nbytes),
+              "ucg_builtin_dev_sum_dropout_grad")
+
+    def _workspace(self, workspace, need, *sizes):
+        """A workspace's address and bytes. An address alone is taken to hold
+        what the call needs, as the C caller says it does."""
+        if workspace is None:
+            return None, 0
+        if isinstance(workspace, int):
+            return workspace, need(*sizes)
+        if hasattr(workspace, "data_ptr"):
+            if workspace.device.type != "cuda" or workspace.device.index != self.device or \
+                    not workspace.is_contiguous():
+                raise ValueError(f"workspace: a contiguous tensor on cuda:{self.device} wanted")
+            return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        return workspace.ptr, workspace.nbytes
+
+    @staticmethod
+    def balance_workspace(tokens, experts):
+        """bytes of balance's workspace"""
+        return _lib.dev().ucg_builtin_dev_balance_workspace(tokens, experts)
+
+    def balance(self, dt, logits, index, tokens, experts, topk, counts, sums, mask=None,
+                loss=None, balance_coef=0.0, z_coef=0.0, index_dt="int64", ld=0, ld_index=0,
+                workspace=None):
+        """counts (experts + 1 int64: uses of each expert, tokens) and sums
+        (experts + 1 float32: probability of each expert, squared log sum exp)
+        of this member's tokens: what the group adds up
+        (ucg_builtin_dev_balance). loss: 3 floats, for a group of one."""
+        dt, index_dt = _name(dt), _name(index_dt)
+        logits, index, mask, counts, sums, loss = self._operands(
+            ("logits", logits, dt, (tokens, experts), ld or experts),
+            ("index", index, index_dt, (tokens, topk), ld_index or topk),
+            ("mask", mask, "uint8", (tokens,), tokens),
+            ("counts", counts, "int64", (experts + 1,), None),
+            ("sums", sums, "float32", (experts + 1,), None),
+            ("loss", loss, "float32", (3,), None))
+        q = _lib.BalanceParams(_DT[dt], _DT[index_dt], tokens, experts, topk, ld, ld_index, 0,
+                               balance_coef, z_coef)
+        ws, nbytes = self._workspace(workspace, self.balance_workspace, tokens, experts)
+        check(_lib.dev().ucg_builtin_dev_balance(self.handle, q, logits, index, mask, counts,
+                                                 sums, loss, ws, nbytes),
+              "ucg_builtin_dev_balance")
+
+    def balance_loss(self, counts, sums, experts, topk, loss, balance_coef=0.0, z_coef=0.0):
+        """loss (3 floats: whole, balance part, z part) from the group's counts
+        and sums (ucg_builtin_dev_balance_loss)."""
+        counts, sums, loss = self._operands(("counts", counts, "int64", (experts + 1,), None),
+                                            ("sums", sums, "float32", (experts + 1,), None),
+                                            ("loss", loss, "float32", (3,), None))
+        q = _lib.BalanceParams(_DT["float32"], _DT["int64"], 0, experts, topk, 0, 0, 0,
+                               balance_coef, z_coef)
+        check(_lib.dev().ucg_builtin_dev_balance_loss(self.handle, q, counts, sums, loss),
+              "ucg_builtin_dev_balance_loss")
+
+    def balance_grad(self, dt, dlogits, logits, tokens, experts, topk, counts, mask=None,
+                     base=None, grad_loss=None, balance_coef=0.0, z_coef=0.0, ld=0, ld_out=0):
+        """dlogits = base + grad_loss * the loss' gradient, with the group's
+        counts (ucg_builtin_dev_balance_grad)."""
+        dt = _name(dt)
+        dlogits, logits, mask, counts, base, grad_loss = self._operands(
+            ("dlogits", dlogits, dt, (tokens, experts), ld_out or experts),
+            ("logits", logits, dt, (tokens, experts), ld or experts),
+            ("mask", mask, "uint8", (tokens,), tokens),
+            ("counts", counts, "int64", (experts + 1,), None),
+            ("base", base, dt, (tokens, experts), ld_out or experts),
+            ("grad_loss", grad_loss, "float32", (1,), None))
+        q = _lib.BalanceParams(_DT[dt], _DT["int64"], tokens, experts, topk, ld, 0, ld_out,
+                               balance_coef, z_coef)
+        check(_lib.dev().ucg_builtin_dev_balance_grad(self.handle, q, logits, mask, counts, base,
+                                                      grad_loss, dlogits),
+              "ucg_builtin_dev_balance_grad")
+
+    @staticmethod
+    def policy_workspace(rows, cols):
+        """bytes of policy's workspace"""
+        return _lib.dev().ucg_builtin_dev_policy_workspace(rows, cols)
+
+    def policy(self, dt, logp, old, adv, rows, cols, sums, counts, ref=None, mask=None,
+               row_tokens=None, adv_per_row=False, per_sequence=False, clip_low=0.2,
+               clip_high=0.2, kl_coef=0.0, loss=None, ld=0, workspace=None):
+        """sums (2 float32: clipped policy term, KL) and counts (3 int64:
+        tokens, rows that have one, cut tokens) of this member's answers: what
+        the group adds up (ucg_builtin_dev_policy). loss: 3 floats, for a group
+        of one."""
+        dt, shape, step = _name(dt), (rows, cols), ld or cols
+        logp, old, ref, adv, mask, sums, counts, row_tokens, loss = self._operands(
+            ("logp", logp, dt, shape, step), ("old", old, dt, shape, step),
+            ("ref", ref, dt, shape, step),
+            ("adv", adv, "float32", (rows,) if adv_per_row else shape,
+             rows if adv_per_row else step),
+            ("mask", mask, "uint8", shape, step), ("sums", sums, "float32", (2,), None),
+            ("counts", counts, "int64", (3,), None),
+            ("row_tokens", row_tokens, "int32", (rows,), None),
+            ("loss", loss, "float32", (3,), None))
+        q = _lib.PolicyParams(_DT[dt], adv_per_row, per_sequence, rows, cols, ld, clip_low,
+                              clip_high, kl_coef)
+        ws, nbytes = self._workspace(workspace, self.policy_workspace, rows, cols)
+        check(_lib.dev().ucg_builtin_dev_policy(self.handle, q, logp, old, ref, adv, mask, sums,
+                                                counts, row_tokens, loss, ws, nbytes),
+              "ucg_builtin_dev_policy")
+
+    def policy_loss(self, sums, counts, loss, per_sequence=False, kl_coef=0.0):
+        """loss (3 floats: whole, policy mean, KL mean) from the group's sums
+        and counts (ucg_builtin_dev_policy_loss)."""
+        sums, counts, loss = self._operands(("sums", sums, "float32", (2,), None),
+                                            ("counts", counts, "int64", (3,), None),
+                                            ("loss", loss, "float32", (3,), None))
+        q = _lib.PolicyParams(_DT["float32"], 0, per_sequence, 0, 0, 0, 0.0, 0.0, kl_coef)
+        check(_lib.dev().ucg_builtin_dev_policy_loss(self.handle, q, sums, counts, loss),
+              "ucg_builtin_dev_policy_loss")
+
+    def policy_grad(self, dt, dlogp, logp, old, adv, rows, cols, counts, ref=None, mask=None,
+                    row_tokens=None, adv_per_row=False, per_sequence=False, clip_low=0.2,
+                    clip_high=0.2, kl_coef=0.0, grad_loss=None, ld=0):
+        """dlogp = grad_loss * the loss' gradient, with the group's counts
+        (ucg_builtin_dev_policy_grad)."""
+        dt, shape, step = _name(dt), (rows, cols), ld or cols
+        dlogp, logp, old, ref, adv, mask, row_tokens, counts, grad_loss = self._operands(
+            ("dlogp", dlogp, dt, shape, step), ("logp", logp, dt, shape, step),
+            ("old", old, dt, shape, step), ("ref", ref, dt, shape, step),
+            ("adv", adv, "float32", (rows,) if adv_per_row else shape,
+             rows if adv_per_row else step),
+            ("mask", mask, "uint8", shape, step),
+            ("row_tokens", row_tokens, "int32", (rows,), None),
+            ("counts", counts, "int64", (3,), None),
+            ("grad_loss", grad_loss, "float32", (1,), None))
+        q = _lib.PolicyParams(_DT[dt], adv_per_row, per_sequence, rows, cols, ld, clip_low,
+                              clip_high, kl_coef)
+        check(_lib.dev().ucg_builtin_dev_policy_grad(self.handle, q, logp, old, ref, adv, mask,
+                                                     row_tokens, counts, grad_loss, dlogp),
+              "ucg_builtin_dev_policy_grad")
 
     def combine_host(self, op, dt, dst_host, src_host, count):
         return _lib.dev().ucg_builtin_dev_combine_host(self.handle, op_index(op),

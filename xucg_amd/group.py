@@ -422,3 +422,60 @@ def stream_barrier(dist, device, group=None):
     def barrier():
         dist.all_reduce(flag, group=group)
     return barrier
+
+
+# ---- a training step's operators over a group --------------------------------
+def row_bounds(rows, world, rank):
+    """[lo, hi) rows of `rank`'s shard of a rows x cols tensor: whole rows, the
+    first rows % world members one more."""
+    if world <= 0 or not 0 <= rank < world:
+        raise ValueError("bad rank/world")
+    per, more = divmod(rows, world)
+    lo = rank * per + min(rank, more)
+    return lo, lo + per + (rank < more)
+
+
+def oneshot_reduce_scatter_dropout(ctx, peers, out_ptr, rows, cols, dt, p, seed, rank, world,
+                                   tag=0, offset=0, bias=None, residual=None, out_dt=None,
+                                   rng=None):
+    """oneshot_reduce_scatter by rows with a tensor-parallel block's epilogue:
+    out = residual + dropout(sum over the members of their rows [lo, hi) +
+    bias), read in place through `peers` in one launch
+    (ucg_builtin_dev_sum_dropout). out and residual are this member's rows; the
+    mask is that of the whole tensor, whose first element has place `offset`.
+    The barriers are oneshot_reduce_scatter's. Returns (lo, hi)."""
+    size = _lib.DTYPE_SIZE[_lib.dt_index(dt)]
+    lo, hi = row_bounds(rows, world, rank)
+    ctx.sum_dropout(dt, out_ptr, [q + lo * cols * size for q in peers.ptrs], hi - lo, cols, p,
+                    seed, tag=tag, offset=offset + lo * cols, bias=bias, residual=residual,
+                    out_dt=out_dt, rng=rng)
+    return lo, hi
+
+
+def group_balance(ctx, allreduce, dt, logits, index, tokens, experts, topk, counts, sums, loss,
+                  mask=None, balance_coef=0.0, z_coef=0.0, index_dt="int64", ld=0, ld_index=0,
+                  workspace=None):
+    """The balance loss over a group: this member's statistics, summed over the
+    members, then the loss, the same on every member. counts then holds what
+    DevContext.balance_grad takes. allreduce(buf, dt, count) sums a buffer over
+    the members in place, ordered behind the context's stream
+    (torch.distributed's all_reduce over RCCL on it, or oneshot_allreduce)."""
+    ctx.balance(dt, logits, index, tokens, experts, topk, counts, sums, mask=mask,
+                index_dt=index_dt, ld=ld, ld_index=ld_index, workspace=workspace)
+    allreduce(counts, "int64", experts + 1)
+    allreduce(sums, "float32", experts + 1)
+    ctx.balance_loss(counts, sums, experts, topk, loss, balance_coef=balance_coef, z_coef=z_coef)
+
+
+def group_policy(ctx, allreduce, dt, logp, old, adv, rows, cols, sums, counts, loss, ref=None,
+                 mask=None, row_tokens=None, adv_per_row=False, per_sequence=False, clip_low=0.2,
+                 clip_high=0.2, kl_coef=0.0, ld=0, workspace=None):
+    """The clipped policy loss over a group: as group_balance, with counts (and
+    row_tokens, which stay this member's) for DevContext.policy_grad."""
+    ctx.policy(dt, logp, old, adv, rows, cols, sums, counts, ref=ref, mask=mask,
+               row_tokens=row_tokens, adv_per_row=adv_per_row, per_sequence=per_sequence,
+               clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, ld=ld,
+               workspace=workspace)
+    allreduce(sums, "float32", 2)
+    allreduce(counts, "int64", 3)
+    ctx.policy_loss(sums, counts, loss, per_sequence=per_sequence, kl_coef=kl_coef)
