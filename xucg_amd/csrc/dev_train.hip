@@ -43,14 +43,19 @@ __device__ __forceinline__ void load_raw(const T *p, T (&o)[V])
     __builtin_memcpy(o, &w, sizeof(o));
 }
 
+/* elements [c, c + V) of a row of n, `fill` past its end. The values stay as
+ * they were loaded: a conversion here would wait for them, and the loads that
+ * a caller issues next would not be in flight together. */
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T *p, float (&o)[V])
+__device__ __forceinline__ void load_row(const T *row, uint64_t c, uint64_t n, T fill, T (&o)[V])
 {
-    T t[V];
-    load_raw<T, V>(p, t);
+    if (c + V <= n) {
+        load_raw<T, V>(row + c, o);
+    } else {
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-        o[k] = (float)t[k];
+        for (int k = 0; k < V; k++) {
+            o[k] = c + k < n ? row[c + k] : fill;
+        }
     }
 }
 
@@ -66,21 +71,6 @@ __device__ __forceinline__ void store_vec(T *p, const float (&x)[V])
     W w;
     __builtin_memcpy(&w, t, sizeof(w));
     __builtin_nontemporal_store(w, reinterpret_cast<W*>(p));
-}
-
-/* elements [c, c + V) of a row of n, `fill` past its end */
-template <typename T, int V>
-__device__ __forceinline__ void load_row(const T *row, size_t c, size_t n, float fill,
-                                         float (&o)[V])
-{
-    if (c + V <= n) {
-        load_vec<T, V>(row + c, o);
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            o[k] = c + k < n ? (float)row[c + k] : fill;
-        }
-    }
 }
 
 template <typename T, int V>
@@ -131,11 +121,15 @@ __device__ __forceinline__ float group_all(float x, F f)
     if constexpr (G >= 16) {
         x = f(x, dpp<0x140>(x));      /* row_mirror */
     }
-    if constexpr (G >= 32) {
-        x = f(x, __shfl_xor(x, 16, 64));
+    if constexpr (G >= 32) {          /* rows 0, 2 beside rows 1, 3 */
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
     }
-    if constexpr (G >= 64) {
-        x = f(x, __shfl_xor(x, 32, 64));
+    if constexpr (G >= 64) {          /* the lower half beside the upper */
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x),
+                                                        false, false);
+        x = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
     }
     return x;
 }
@@ -148,9 +142,8 @@ struct Max {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
 
-/* sum over the block's 256 threads in thread order of halves; every thread
- * calls it, thread 0 has the result */
-template <typename X>
+/* sum over the block's NT threads, in every thread; lds holds NT / 64 values */
+template <int NT, typename X>
 __device__ __forceinline__ X block_sum(X x, X *lds)
 {
     x = lanes_all(x, 1, 64, Add());
@@ -159,7 +152,12 @@ __device__ __forceinline__ X block_sum(X x, X *lds)
         lds[threadIdx.x >> 6] = x;
     }
     __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) {
+        x += lds[w];
+    }
+    return x;
 }
 
 /* True in every thread of the last block to arrive, with the other blocks'
@@ -190,10 +188,10 @@ struct Rng {
     float           scale;
 };
 
-/* Philox-4x32-10 for counter (group, tag): eight 16-bit numbers. One round is
- * two 32 x 32 -> 64 bit products and two three-way xors; ten rounds for eight
- * elements keep it below the time the elements' own bytes take (a 32-bit
- * number for each element would double it). */
+/* Philox-4x32-10 for counter (group, tag): eight 16-bit numbers. A round is two
+ * 32 x 32 -> 64 bit products and two three-way xors (bitop3 0x96), 40
+ * instructions in all for eight elements; a 32-bit number for each element
+ * would take twice that and leave the bandwidth. */
 __device__ __forceinline__ void philox(uint64_t group, uint64_t tag, uint64_t seed,
                                        uint32_t (&w)[4])
 {
@@ -203,9 +201,9 @@ __device__ __forceinline__ void philox(uint64_t group, uint64_t tag, uint64_t se
 #pragma unroll
     for (int r = 0; r < 10; r++) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), c1, k0, 0x96);
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), c3, k1, 0x96);
         c3 = (uint32_t)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
@@ -226,217 +224,236 @@ __device__ __forceinline__ void rng_state(const Rng &r, uint64_t &seed, uint64_t
     }
 }
 
-/* the 16-bit numbers of elements [at, at + V) of the tensor, two to a word.
- * ALIGNED: at is a multiple of V, so they lie in one group of eight. */
-template <int V, bool ALIGNED>
-__device__ __forceinline__ void draw(uint64_t at, uint64_t tag, uint64_t seed,
-                                     uint32_t (&o)[V / 2])
+/* the 16-bit numbers of elements [at, at + 8) of the tensor, two to a word.
+ * ALIGNED: at is a multiple of 8, so they are one group. */
+template <bool ALIGNED>
+__device__ __forceinline__ void draw(uint64_t at, uint64_t tag, uint64_t seed, uint32_t (&o)[4])
 {
-    uint32_t w[4];
-    philox(at >> 3, tag, seed, w);
-    const unsigned sub = (unsigned)at & 7;
-    if constexpr (ALIGNED && V == 8) {
+    philox(at >> 3, tag, seed, o);
+    if constexpr (!ALIGNED) {
+        uint32_t w[4];
+        philox((at >> 3) + 1, tag, seed, w);
+        uint32_t x[8] = {o[0], o[1], o[2], o[3], w[0], w[1], w[2], w[3]};
+        const unsigned sub = (unsigned)at & 7;
+        /* shift the eight words right by sub halves; by masks, since a choice
+         * between two of the array's places would put it into scratch memory */
+        const uint32_t by2 = 0u - ((sub >> 2) & 1), by1 = 0u - ((sub >> 1) & 1);
+#pragma unroll
+        for (int k = 0; k < 6; k++) {
+            x[k] ^= (x[k] ^ x[k + 2]) & by2;
+        }
+#pragma unroll
+        for (int k = 0; k < 5; k++) {
+            x[k] ^= (x[k] ^ x[k + 1]) & by1;
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            o[k] = w[k];
-        }
-    } else if constexpr (ALIGNED) {
-        static_assert(V == 4, "a vector is a group or half of one");
-        o[0] = sub ? w[2] : w[0];
-        o[1] = sub ? w[3] : w[1];
-    } else {
-        uint32_t x[9] = {w[0], w[1], w[2], w[3], 0, 0, 0, 0, 0};
-        if (sub + V > 8) {
-            philox((at >> 3) + 1, tag, seed, w);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                x[4 + k] = w[k];
-            }
-        }
-        /* shift the eight words right by sub halves */
-#pragma unroll
-        for (int k = 0; k < 6; k++) {
-            x[k] = sub & 4 ? x[k + 2] : x[k];
-        }
-#pragma unroll
-        for (int k = 0; k < 6; k++) {
-            x[k] = sub & 2 ? x[k + 1] : x[k];
-        }
-#pragma unroll
-        for (int k = 0; k < V / 2; k++) {
-            o[k] = sub & 1 ? (x[k] >> 16) | (x[k + 1] << 16) : x[k];
+            o[k] = __builtin_amdgcn_alignbit(x[k + 1], x[k], 16 * (sub & 1));
         }
     }
 }
 
-template <int V>
-__device__ __forceinline__ bool kept(const uint32_t (&u)[V / 2], int k, uint32_t threshold)
+/* 16-bit number k of the words */
+__device__ __forceinline__ bool kept(const uint32_t *u, int k, uint32_t threshold)
 {
     return ((u[k >> 1] >> (16 * (k & 1))) & 0xffffu) >= threshold;
 }
 
-/* N > 0: that many sources, in registers at once; 0: any number, one by one */
-template <typename T, int N, typename L>
-__device__ __forceinline__ float sum_sources(const SrcList &srcs, unsigned nsrc, L at)
+/* the sum of N values as the combine associates it */
+template <int N>
+__device__ __forceinline__ float sum_of(float (&v)[N])
 {
-    if constexpr (N == 0) {
-        float s = at(static_cast<const T*>(srcs.p[0]));
-        for (unsigned m = 1; m < nsrc; m++) {
-            s = at(static_cast<const T*>(srcs.p[m])) + s;
+    if constexpr ((N & (N - 1)) == 0) {
+        return rd_tree<N>(v, Add());
+    } else {
+        float s = v[0];
+#pragma unroll
+        for (int m = 1; m < N; m++) {
+            s = v[m] + s;
         }
         return s;
-    } else {
-        float v[N];
-#pragma unroll
-        for (int m = 0; m < N; m++) {
-            v[m] = at(static_cast<const T*>(srcs.p[m]));
-        }
-        if constexpr ((N & (N - 1)) == 0) {
-            return rd_tree<N>(v, Add());
-        } else {
-            float s = v[0];
-#pragma unroll
-            for (int m = 1; m < N; m++) {
-                s = v[m] + s;
-            }
-            return s;
-        }
     }
 }
 
+/* elements of a wave, eight to a lane: one Philox group each */
+constexpr int kWaveElems = 512;
+
 /*
- * One lane does the V elements whose place in the whole tensor starts at a
- * multiple of V, so that one Philox group serves them; the first and the last
- * lane of a call may have fewer and go element by element. `inv` is
- * 2^64 / cols rounded up (unused for one column): the quotient by cols is its
- * high product, or one less (the rounding adds i * e / 2^64 < 1 with e <= 1).
+ * A wave does 512 neighbouring elements that start at a multiple of eight in
+ * the whole tensor, a lane computes one group of eight numbers. With 16-bit
+ * operands alone (V = 8) the group is the lane's own vector. With a 32-bit
+ * operand a 16-byte vector is four elements: the wave has two tiles of 64
+ * vectors, even lanes compute a group of the first tile and odd lanes one of
+ * the second, and each hands its neighbour the half that it needs. (Half a
+ * group used by each lane instead costs a second Philox: 234 against 2xx us.)
+ * N operands (0: nsrc of them, one by one) and the residual are all in flight
+ * before the numbers are computed.
+ *
+ * `inv` is 2^64 / cols rounded up (unused for one column): the quotient by
+ * cols is its high product, or one less (the rounding adds i * e / 2^64 < 1
+ * with e <= 1).
  */
-template <typename T, typename R, int V, int N>
+template <typename T, typename R, int N>
 __global__ void __launch_bounds__(kThreads)
 k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *residual,
               uint64_t n, uint64_t first, uint64_t cols, uint64_t inv, Rng rng)
 {
-    const unsigned phase = (unsigned)(rng.offset % V);
-    const uint64_t g     = first + (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t  i     = (int64_t)(g * V) - phase;
-    if (i >= (int64_t)n) {
+    constexpr int V = sizeof(T) == 2 && sizeof(R) == 2 ? 8 : 4, TL = 8 / V, NN = N ? N : 1;
+    const unsigned phase = (unsigned)(rng.offset % 8);
+    const unsigned lane  = threadIdx.x & 63;
+    const uint64_t wave  = first + (uint64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const int64_t  begin = (int64_t)(wave * kWaveElems) - phase;     /* the wave's first */
+    if (begin >= (int64_t)n) {
         return;
     }
-    uint64_t seed, tag;
-    rng_state(rng, seed, tag);
-    uint32_t u[V / 2] = {};
-    const uint64_t at = rng.offset - phase + g * V;
-    uint64_t col = 0;
-    if (bias != nullptr) {
-        const uint64_t j = i > 0 ? (uint64_t)i : 0;
-        const uint64_t q = __umul64hi(j, inv);
-        col = j - q * cols;
-        col = cols == 1 ? 0 : (int64_t)col < 0 ? col + cols : col;
-    }
-    if (i >= 0 && i + V <= (int64_t)n) {
-        float s[V];
-        if constexpr (N == 0) {
-            load_vec<T, V>(static_cast<const T*>(srcs.p[0]) + i, s);
-#pragma unroll 4
-            for (unsigned m = 1; m < nsrc; m++) {
-                float x[V];
-                load_vec<T, V>(static_cast<const T*>(srcs.p[m]) + i, x);
+    const int64_t i = begin + (int64_t)lane * V;         /* of the lane's first tile */
+    const bool whole = i >= 0 && i + (TL - 1) * 64 * V + V <= (int64_t)n;
+
+    T x[NN][TL][V];
+    R r[TL][V];
+    if (whole) {
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    s[k] = x[k] + s[k];
-                }
+        for (int m = 0; m < NN; m++) {
+#pragma unroll
+            for (int j = 0; j < TL; j++) {
+                load_raw<T, V>(static_cast<const T*>(srcs.p[m]) + i + j * 64 * V, x[m][j]);
+            }
+        }
+        if (residual != nullptr) {
+#pragma unroll
+            for (int j = 0; j < TL; j++) {
+                load_raw<R, V>(residual + i + j * 64 * V, r[j]);
+            }
+        }
+    }
+
+    uint32_t u[TL][V / 2] = {};
+    if (rng.threshold != 0) {
+        uint64_t seed, tag;
+        rng_state(rng, seed, tag);
+        const uint64_t group = (rng.offset - phase) / 8 + wave * (kWaveElems / 8);
+        uint32_t w[4];
+        if constexpr (V == 8) {
+            philox(group + lane, tag, seed, w);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                u[0][k] = w[k];
             }
         } else {
-            float x[N][V];
+            const bool odd = lane & 1;
+            philox(group + (odd ? 32 : 0) + lane / 2, tag, seed, w);
+            /* an even lane keeps the lower half of its group, an odd one the upper */
 #pragma unroll
-            for (int m = 0; m < N; m++) {
-                load_vec<T, V>(static_cast<const T*>(srcs.p[m]) + i, x[m]);
+            for (int k = 0; k < 2; k++) {
+                const uint32_t mine = odd ? w[2 + k] : w[k];
+                const uint32_t give = odd ? w[k] : w[2 + k];
+                const uint32_t got  = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xB1, 0xf, 0xf,
+                                                                         true);
+                u[0][k]      = odd ? got : mine;
+                u[TL - 1][k] = odd ? mine : got;
             }
+        }
+    }
+
+#pragma unroll
+    for (int j = 0; j < TL; j++) {
+        const int64_t at = i + j * 64 * V;
+        uint64_t col = 0;
+        if (bias != nullptr) {
+            const uint64_t a = at > 0 ? (uint64_t)at : 0;
+            col = a - __umul64hi(a, inv) * cols;
+            col = cols == 1 ? 0 : (int64_t)col < 0 ? col + cols : col;
+        }
+        if (whole) {
+            float s[V];
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                float v[N];
+                float v[NN];
 #pragma unroll
-                for (int m = 0; m < N; m++) {
-                    v[m] = x[m][k];
+                for (int m = 0; m < NN; m++) {
+                    v[m] = (float)x[m][j][k];
                 }
-                if constexpr ((N & (N - 1)) == 0) {
-                    s[k] = rd_tree<N>(v, Add());
-                } else {
-                    s[k] = v[0];
+                s[k] = sum_of<NN>(v);
+            }
+            if constexpr (N == 0) {
+#pragma unroll 4
+                for (unsigned m = 1; m < nsrc; m++) {
+                    T y[V];
+                    load_raw<T, V>(static_cast<const T*>(srcs.p[m]) + at, y);
 #pragma unroll
-                    for (int m = 1; m < N; m++) {
-                        s[k] = v[m] + s[k];
+                    for (int k = 0; k < V; k++) {
+                        s[k] = (float)y[k] + s[k];
                     }
                 }
             }
-        }
-        float r[V] = {};
-        if (residual != nullptr) {
-            load_vec<R, V>(residual + i, r);
-        }
-        if (bias != nullptr) {
-            float b[V];
-            if (col + V <= cols) {
-                T t[V];
-                __builtin_memcpy(t, bias + col, sizeof(t));   /* temporal: read by every row */
+            if (bias != nullptr) {
+                if (col + V <= cols) {
+                    T b[V];
+                    __builtin_memcpy(b, bias + col, sizeof(b));  /* temporal: every row's */
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    b[k] = (float)t[k];
-                }
-            } else {
-                uint64_t c = col;
+                    for (int k = 0; k < V; k++) {
+                        s[k] += (float)b[k];
+                    }
+                } else {
+                    uint64_t c = col;
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    b[k] = (float)bias[c];
-                    c = c + 1 == cols ? 0 : c + 1;
+                    for (int k = 0; k < V; k++) {
+                        s[k] += (float)bias[c];
+                        c = c + 1 == cols ? 0 : c + 1;
+                    }
                 }
             }
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                s[k] += b[k];
+                const float d = kept(u[j], k, rng.threshold) ? s[k] * rng.scale : 0.f;
+                s[k] = residual != nullptr ? d + (float)r[j][k] : d;
             }
-        }
-        if (rng.threshold != 0) {
-            draw<V, true>(at, tag, seed, u);
-        }
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            const float d = kept<V>(u, k, rng.threshold) ? s[k] * rng.scale : 0.f;
-            s[k] = residual != nullptr ? d + r[k] : d;
-        }
-        store_vec<R, V>(dst + i, s);
-        return;
-    }
-    if (rng.threshold != 0) {
-        draw<V, true>(at, tag, seed, u);
-    }
-    for (int k = 0; k < V; k++) {
-        const int64_t j = i + k;
-        if (j < 0 || j >= (int64_t)n) {
+            store_vec<R, V>(dst + at, s);
             continue;
         }
-        float s = sum_sources<T, N>(srcs, nsrc, [&](const T *p) { return (float)p[j]; });
-        if (bias != nullptr) {
-            s += (float)bias[col];
-            col = col + 1 == cols ? 0 : col + 1;
+        for (int k = 0; k < V; k++) {
+            const int64_t e = at + k;
+            if (e < 0 || e >= (int64_t)n) {
+                continue;
+            }
+            float s;
+            if constexpr (N == 0) {
+                s = (float)static_cast<const T*>(srcs.p[0])[e];
+                for (unsigned m = 1; m < nsrc; m++) {
+                    s = (float)static_cast<const T*>(srcs.p[m])[e] + s;
+                }
+            } else {
+                float v[N];
+#pragma unroll
+                for (int m = 0; m < N; m++) {
+                    v[m] = (float)static_cast<const T*>(srcs.p[m])[e];
+                }
+                s = sum_of<N>(v);
+            }
+            if (bias != nullptr) {
+                s += (float)bias[col];
+                col = col + 1 == cols ? 0 : col + 1;
+            }
+            const float d = kept(u[j], k, rng.threshold) ? s * rng.scale : 0.f;
+            dst[e] = (R)(residual != nullptr ? d + (float)residual[e] : d);
         }
-        const float d = kept<V>(u, k, rng.threshold) ? s * rng.scale : 0.f;
-        dst[j] = (R)(residual != nullptr ? d + (float)residual[j] : d);
     }
 }
 
 /*
- * The gradient with the bias' part: a lane keeps V columns over the rows of
+ * The gradient with the bias' part: a lane keeps eight columns over the rows of
  * its chunk, tx lanes side by side and kThreads / tx rows at once, and the
- * block's rows are joined in LDS. A row may start anywhere in a group of eight
- * (ALIGNED 0: the columns or the offset are no multiple of V): then V numbers
+ * block's rows are joined in LDS. Four rows are loaded while the four before
+ * them are computed. A row may start anywhere in a group of eight (ALIGNED 0:
+ * the columns or the offset are no multiple of eight): then a lane's numbers
  * come from two groups.
  */
-template <typename R, typename T, int V, bool ALIGNED>
+template <typename R, typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t cols,
                unsigned tx, uint64_t chunk, Rng rng)
 {
+    constexpr int V = 8, U = 4;
     __shared__ float lds[kThreads * V];
     const unsigned x  = threadIdx.x % tx, y = threadIdx.x / tx, ty = kThreads / tx;
     const uint64_t c  = ((uint64_t)blockIdx.x * tx + x) * V;
@@ -445,31 +462,53 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
     uint64_t seed, tag;
     rng_state(rng, seed, tag);
     float sum[V] = {};
-    if (c < cols) {
-        constexpr int U = 4;          /* rows in flight */
-        for (uint64_t r = r0 + y; r < r1; r += (uint64_t)U * ty) {
-            float g[U][V];
+    if (c + V <= cols && r0 + y < r1) {
+        const uint64_t last = r1 - 1;
+        R g[U][V];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const uint64_t q = r0 + y + (uint64_t)j * ty;
+            load_raw<R, V>(grad + (q < r1 ? q : last) * cols + c, g[j]);
+        }
+        for (uint64_t row = r0 + y; row < r1; row += (uint64_t)U * ty) {
+            R next[U][V];
 #pragma unroll
             for (int j = 0; j < U; j++) {
-                const uint64_t q = r + (uint64_t)j * ty;
-                if (q < r1) {
-                    load_row<R, V>(grad + q * cols, c, cols, 0.f, g[j]);
-                }
+                const uint64_t q = row + (uint64_t)(U + j) * ty;
+                load_raw<R, V>(grad + (q < r1 ? q : last) * cols + c, next[j]);
             }
 #pragma unroll
             for (int j = 0; j < U; j++) {
-                const uint64_t q = r + (uint64_t)j * ty;
+                const uint64_t q = row + (uint64_t)j * ty;
                 if (q < r1) {
-                    uint32_t u[V / 2] = {};
+                    uint32_t u[4] = {};
                     if (rng.threshold != 0) {
-                        draw<V, ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
+                        draw<ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
                     }
+                    float d[V];
 #pragma unroll
                     for (int k = 0; k < V; k++) {
-                        g[j][k] = kept<V>(u, k, rng.threshold) ? g[j][k] * rng.scale : 0.f;
-                        sum[k] += g[j][k];
+                        d[k] = kept(u, k, rng.threshold) ? (float)g[j][k] * rng.scale : 0.f;
+                        sum[k] += d[k];
                     }
-                    store_row<T, V>(dsrc + q * cols, c, cols, g[j]);
+                    store_vec<T, V>(dsrc + q * cols + c, d);
+                }
+            }
+            __builtin_memcpy(g, next, sizeof(g));
+        }
+    } else if (c < cols) {
+        for (uint64_t q = r0 + y; q < r1; q += ty) {
+            uint32_t u[4] = {};
+            if (rng.threshold != 0) {
+                draw<ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (c + k < cols) {
+                    const float d = kept(u, k, rng.threshold)
+                                        ? (float)grad[q * cols + c + k] * rng.scale : 0.f;
+                    sum[k] += d;
+                    dsrc[q * cols + c + k] = (T)d;
                 }
             }
         }
@@ -492,23 +531,33 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
     }
 }
 
-/* 16 columns by 16 parts of the partials' rows */
+constexpr unsigned kMaxParts = 256;    /* partials to join */
+
+/* 16 columns by 16 parts of the partials' rows (at most kMaxParts of them, so
+ * that a lane's loads are all in flight at once); the sum in every thread of
+ * the column */
 template <typename X, typename S>
-__device__ __forceinline__ S join_columns(const X *part, uint64_t nparts, uint64_t stride,
+__device__ __forceinline__ S join_columns(const X *part, unsigned nparts, uint64_t stride,
                                           uint64_t col, uint64_t cols, S *lds)
 {
     const unsigned x = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const X *at = part + (col < cols ? col : cols - 1);
+    X v[kMaxParts / 16];
+#pragma unroll
+    for (unsigned j = 0; j < kMaxParts / 16; j++) {
+        const unsigned p = y + j * 16;
+        v[j] = at[(p < nparts ? p : nparts - 1) * stride];
+    }
     S s = 0;
-    if (col < cols) {
-#pragma unroll 8
-        for (uint64_t p = y; p < nparts; p += 16) {
-            s += (S)part[p * stride + col];
-        }
+#pragma unroll
+    for (unsigned j = 0; j < kMaxParts / 16; j++) {
+        s += y + j * 16 < nparts ? (S)v[j] : (S)0;
     }
     __syncthreads();
     lds[threadIdx.x] = s;
     __syncthreads();
     S t = 0;
+#pragma unroll
     for (unsigned q = 0; q < 16; q++) {
         t += lds[q * 16 + x];
     }
@@ -516,7 +565,7 @@ __device__ __forceinline__ S join_columns(const X *part, uint64_t nparts, uint64
 }
 
 __global__ void __launch_bounds__(kThreads)
-k_join_bias(float *dbias, const float *part, uint64_t nparts, uint64_t cols)
+k_join_bias(float *dbias, const float *part, unsigned nparts, uint64_t cols)
 {
     __shared__ double lds[kThreads];
     const uint64_t col = (uint64_t)blockIdx.x * 16 + (threadIdx.x & 15);
@@ -561,16 +610,17 @@ __device__ __forceinline__ void row_softmax(float (&x)[C], float &inv, float &ls
     lse = none ? 0.f : __builtin_fmaf(__builtin_amdgcn_logf(sum), kLn2, top);
 }
 
-/* the loss' three values from whole counts and sums, by one block */
+/* the loss' three values from whole counts and sums, by one block of NT */
+template <int NT>
 __device__ __forceinline__ void balance_loss_block(const int64_t *counts, const float *sums,
                                                    unsigned experts, double balance,
                                                    double z_coef, float *loss, double *lds)
 {
     double dot = 0;
-    for (unsigned e = threadIdx.x; e < experts; e += kThreads) {
+    for (unsigned e = threadIdx.x; e < experts; e += NT) {
         dot += (double)counts[e] * (double)sums[e];
     }
-    dot = block_sum(dot, lds);
+    dot = block_sum<NT>(dot, lds);
     if (threadIdx.x == 0) {
         const double n = (double)counts[experts];
         const double b = n > 0 ? balance * dot / (n * n) : 0;
@@ -597,23 +647,52 @@ struct BalancePart {
     unsigned *done;
 };
 
+/* columns [c, c + V) of a row of E logits, -inf past its end. EVEN: E is a
+ * multiple of V, so that a lane has a whole vector or none. */
+template <typename T, int V, bool EVEN>
+__device__ __forceinline__ void load_logits(const T *row, unsigned c, unsigned E, T (&o)[V])
+{
+    if constexpr (EVEN) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            o[k] = (T)-INFINITY;
+        }
+        if (c < E) {
+            load_raw<T, V>(row + c, o);
+        }
+    } else {
+        load_row<T, V>(row, c, E, (T)-INFINITY, o);
+    }
+}
+
+/* rows of a lane group in flight at once: what 16 to 32 registers of values hold */
+template <int NV>
+constexpr int rows_at_once()
+{
+    return NV == 1 ? 4 : NV == 2 ? 2 : 1;
+}
+
+constexpr int kBalanceThreads = 1024;  /* 16 waves: one block to a CU */
+
 /* A row lies in G lanes, V neighbouring columns to a lane and vector, so a
- * wave has 64 / G rows at once and a lane keeps the sums of its columns over
- * all rows of the block. Counts are integers, so their LDS atomics give the
- * same in any order. */
-template <typename T, typename I, int G, int NV>
-__global__ void __launch_bounds__(kThreads)
+ * wave has 64 / G rows at once, U such sets in flight, and a lane keeps the sums
+ * of its columns over all rows of the block. A masked row is loaded like the
+ * others (the mask is not waited for) and left out afterwards. Counts are
+ * integers, so their LDS atomics give the same in any order. */
+template <typename T, typename I, int G, int NV, bool EVEN>
+__global__ void __launch_bounds__(kBalanceThreads)
 k_balance(const T *logits, const I *index, const uint8_t *mask, Balance p, BalancePart out,
           int64_t *counts, float *sums, float *loss)
 {
-    constexpr int V = 16 / sizeof(T), C = NV * V, R = 64 / G;
-    __shared__ float psum[4][G * C + 1];
+    constexpr int V = 16 / sizeof(T), C = NV * V, R = 64 / G, U = rows_at_once<NV>();
+    constexpr int W = kBalanceThreads / 64;
+    __shared__ float psum[W / 2][G * C + 1];
     __shared__ unsigned hist[G * C + 1];
-    __shared__ double join[4];
+    __shared__ double join[W];
     const unsigned E    = p.experts;
     const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const unsigned l    = lane % G, sub = lane / G;
-    for (unsigned e = threadIdx.x; e <= G * C; e += kThreads) {
+    for (unsigned e = threadIdx.x; e <= G * C; e += kBalanceThreads) {
         hist[e] = 0;
     }
     __syncthreads();
@@ -621,34 +700,66 @@ k_balance(const T *logits, const I *index, const uint8_t *mask, Balance p, Balan
     const uint64_t r1 = r0 + p.chunk < p.tokens ? r0 + p.chunk : p.tokens;
     float acc[C] = {}, zsum = 0.f;
     unsigned live_rows = 0;
-    for (uint64_t t = r0 + wave * R + sub; t < r1; t += 4 * R) {
-        if (mask != nullptr && mask[t] == 0) {
-            continue;                 /* the same for a row's G lanes */
-        }
-        float x[C];
+    struct Set {
+        T       raw[U][NV][V];
+        uint8_t on[U];
+        I       named[U];
+    };
+    const auto load = [&](uint64_t t, Set &s) {
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float v[V];
-            load_row<T, V>(logits + t * p.ld, (j * G + l) * V, E, -INFINITY, v);
+        for (int u = 0; u < U; u++) {
+            const uint64_t q = t + (uint64_t)u * W * R;
+            const uint64_t r = q < r1 ? q : r1 - 1;
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                x[j * V + k] = v[k];
+            for (int j = 0; j < NV; j++) {
+                load_logits<T, V, EVEN>(logits + r * p.ld, (j * G + l) * V, E, s.raw[u][j]);
             }
+            s.on[u]    = mask != nullptr ? mask[r] : 1;
+            s.named[u] = l < p.topk ? index[r * p.ld_index + l] : (I)-1;
         }
-        for (unsigned k = l; k < p.topk; k += G) {
-            const int64_t e = (int64_t)index[t * p.ld_index + k];
-            if (e >= 0 && e < (int64_t)E) {
-                atomicAdd(&hist[e], 1u);
-            }
+    };
+    const uint64_t t0 = r0 + wave * R + sub;
+    Set now;
+    if (t0 < r1) {
+        load(t0, now);
+    }
+    for (uint64_t t = t0; t < r1; t += (uint64_t)U * W * R) {
+        Set next;
+        if (t + (uint64_t)U * W * R < r1) {
+            load(t + (uint64_t)U * W * R, next);
         }
-        float inv, lse;
-        row_softmax<G, C>(x, inv, lse);
+        const auto &raw = now.raw;
+        const auto &on = now.on;
+        const auto &named = now.named;
 #pragma unroll
-        for (int k = 0; k < C; k++) {
-            acc[k] = __builtin_fmaf(x[k], inv, acc[k]);
+        for (int u = 0; u < U; u++) {
+            const uint64_t q = t + (uint64_t)u * W * R;
+            if (q >= r1 || on[u] == 0) {      /* the same for a row's G lanes */
+                continue;
+            }
+            if ((int64_t)named[u] >= 0 && (int64_t)named[u] < (int64_t)E) {
+                atomicAdd(&hist[named[u]], 1u);
+            }
+            for (unsigned k = l + G; k < p.topk; k += G) {
+                const int64_t e = (int64_t)index[q * p.ld_index + k];
+                if (e >= 0 && e < (int64_t)E) {
+                    atomicAdd(&hist[e], 1u);
+                }
+            }
+            float x[C], inv, lse;
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                x[k] = (float)raw[u][k / V][k % V];
+            }
+            row_softmax<G, C>(x, inv, lse);
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                acc[k] = __builtin_fmaf(x[k], inv, acc[k]);
+            }
+            zsum = __builtin_fmaf(lse, lse, zsum);
+            live_rows++;
         }
-        zsum = __builtin_fmaf(lse, lse, zsum);
-        live_rows++;
+        now = next;
     }
     /* rows of the wave, then waves, in a fixed order */
 #pragma unroll
@@ -657,21 +768,29 @@ k_balance(const T *logits, const I *index, const uint8_t *mask, Balance p, Balan
     }
     zsum      = lanes_all(zsum, G, 64, Add());
     live_rows = lanes_all(live_rows, G, 64, Add());
-    if (sub == 0) {
+    /* the upper half of the waves hands its sums to the lower: half the LDS */
+    for (int half = 1; half >= 0; half--) {
+        if ((int)(wave / (W / 2)) == half && sub == 0) {
+            float *to = psum[wave % (W / 2)];
 #pragma unroll
-        for (int k = 0; k < C; k++) {
-            psum[wave][((k / V) * G + l) * V + k % V] = acc[k];
+            for (int k = 0; k < C; k++) {
+                const unsigned at = ((k / V) * G + l) * V + k % V;
+                to[at] = half ? acc[k] : to[at] + acc[k];
+            }
+            if (l == 0) {
+                to[G * C] = half ? zsum : to[G * C] + zsum;
+                atomicAdd(&hist[G * C], live_rows);
+            }
         }
+        __syncthreads();
     }
-    if (lane == 0) {
-        psum[wave][G * C] = zsum;
-        atomicAdd(&hist[G * C], live_rows);
-    }
-    __syncthreads();
-    for (unsigned e = threadIdx.x; e <= E; e += kThreads) {
+    for (unsigned e = threadIdx.x; e <= E; e += kBalanceThreads) {
         const unsigned at = e == E ? G * C : e;
-        const double s    = ((double)psum[0][at] + (double)psum[1][at]) +
-                         ((double)psum[2][at] + (double)psum[3][at]);
+        double s = 0;
+#pragma unroll
+        for (int w = 0; w < W / 2; w++) {
+            s += (double)psum[w][at];
+        }
         if (counts != nullptr) {      /* the only block */
             counts[e] = hist[at];
             sums[e]   = (float)s;
@@ -683,7 +802,7 @@ k_balance(const T *logits, const I *index, const uint8_t *mask, Balance p, Balan
     if (counts != nullptr) {
         if (loss != nullptr) {
             __syncthreads();
-            balance_loss_block(counts, sums, E, p.balance, p.z_coef, loss, join);
+            balance_loss_block<kBalanceThreads>(counts, sums, E, p.balance, p.z_coef, loss, join);
         }
     } else if (blockIdx.x == 0 && threadIdx.x == 0) {
         *out.done = 0;
@@ -706,7 +825,7 @@ k_balance_join(BalancePart part, unsigned nparts, Balance p, int64_t *counts, fl
         counts[col] = (int64_t)c;
     }
     if (loss != nullptr && last_block(part.done, &arrived)) {
-        balance_loss_block(counts, sums, p.experts, p.balance, p.z_coef, loss, lds);
+        balance_loss_block<kThreads>(counts, sums, p.experts, p.balance, p.z_coef, loss, lds);
     }
 }
 
@@ -714,77 +833,117 @@ __global__ void __launch_bounds__(kThreads)
 k_balance_loss(const int64_t *counts, const float *sums, Balance p, float *loss)
 {
     __shared__ double lds[4];
-    balance_loss_block(counts, sums, p.experts, p.balance, p.z_coef, loss, lds);
+    balance_loss_block<kThreads>(counts, sums, p.experts, p.balance, p.z_coef, loss, lds);
 }
 
 /* dx_e = grad * p_e ( a (c_e - sum_j p_j c_j) + 2 b lse ), a = balance / N^2,
  * b = z_coef / N. The counts enter less their mean, which the p (that sum to
  * one) cancel: near balance that keeps the digits that the difference needs. */
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, bool EVEN>
 __global__ void __launch_bounds__(kThreads)
 k_balance_grad(const T *logits, const uint8_t *mask, const int64_t *counts, const T *base,
                const float *grad_loss, T *dlogits, Balance p)
 {
-    constexpr int V = 16 / sizeof(T), C = NV * V, R = 64 / G;
+    constexpr int V = 16 / sizeof(T), C = NV * V, R = 64 / G, U = NV == 1 ? 2 : 1;
+    __shared__ float table[G * C];
     const unsigned E    = p.experts;
     const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const unsigned l    = lane % G, sub = lane / G;
+    const uint64_t step = (uint64_t)gridDim.x * 4 * R;
+    struct Set {
+        T       raw[U][NV][V], add[U][NV][V];
+        uint8_t on[U];
+    };
+    const auto load = [&](uint64_t t, Set &s) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint64_t q = t + u * step;
+            const uint64_t r = q < p.tokens ? q : p.tokens - 1;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const unsigned c = (j * G + l) * V;
+                load_logits<T, V, EVEN>(logits + r * p.ld, c, E, s.raw[u][j]);
+                if (base != nullptr) {
+                    load_logits<T, V, EVEN>(base + r * p.ld_out, c, E, s.add[u][j]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V; k++) {
+                        s.add[u][j][k] = (T)0.f;
+                    }
+                }
+            }
+            s.on[u] = mask != nullptr ? mask[r] : 1;
+        }
+    };
+    const uint64_t t0 = ((uint64_t)blockIdx.x * 4 + wave) * R + sub;
+    Set now;
+    if (t0 < p.tokens) {
+        load(t0, now);
+    }
+    /* what a block needs of the counts, once */
     const int64_t tokens = counts[E];
     const int64_t mean   = (int64_t)((double)tokens * p.topk / E);
-    const double g       = grad_loss != nullptr ? (double)*grad_loss : 1.0;
+    for (unsigned e = threadIdx.x; e < G * C; e += kThreads) {
+        table[e] = e < E ? (float)(counts[e] - mean) : 0.f;
+    }
+    const double g = grad_loss != nullptr ? (double)*grad_loss : 1.0;
     const float a = tokens > 0 ? (float)(g * p.balance / ((double)tokens * (double)tokens)) : 0.f;
     const float b = tokens > 0 ? (float)(g * 2 * p.z_coef / (double)tokens) : 0.f;
+    __syncthreads();
     float c[C];
 #pragma unroll
     for (int k = 0; k < C; k++) {
-        const unsigned e = ((k / V) * G + l) * V + k % V;
-        c[k] = e < E ? (float)(counts[e] - mean) : 0.f;
+        c[k] = table[((k / V) * G + l) * V + k % V];
     }
-    for (uint64_t t = ((uint64_t)blockIdx.x * 4 + wave) * R + sub; t < p.tokens;
-         t += (uint64_t)gridDim.x * 4 * R) {
-        const bool live = mask == nullptr || mask[t] != 0;
-        float x[C], d[C];
+    for (uint64_t t = t0; t < p.tokens; t += U * step) {
+        Set next;
+        if (t + U * step < p.tokens) {
+            load(t + U * step, next);
+        }
+        const auto &raw = now.raw;
+        const auto &add = now.add;
+        const auto &on = now.on;
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float v[V] = {}, w[V] = {};
-            if (live) {
-                load_row<T, V>(logits + t * p.ld, (j * G + l) * V, E, -INFINITY, v);
+        for (int u = 0; u < U; u++) {
+            const uint64_t q = t + u * step;
+            if (q >= p.tokens) {              /* the same for a row's G lanes */
+                continue;
             }
-            if (base != nullptr) {
-                load_row<T, V>(base + t * p.ld_out, (j * G + l) * V, E, 0.f, w);
-            }
+            float x[C], inv, lse;
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                x[j * V + k] = live ? v[k] : -INFINITY;
-                d[j * V + k] = w[k];
+            for (int k = 0; k < C; k++) {
+                x[k] = (float)raw[u][k / V][k % V];
+            }
+            row_softmax<G, C>(x, inv, lse);
+            float dot = 0.f;
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                x[k] *= inv;
+                dot = __builtin_fmaf(x[k], c[k], dot);
+            }
+            dot = group_all<G>(dot, Add());
+            const float z = b * lse;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                float d[V];
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    const float w = (float)add[u][j][k];
+                    const float s = __builtin_fmaf(
+                        x[j * V + k], __builtin_fmaf(a, c[j * V + k] - dot, z), w);
+                    d[k] = on[u] != 0 ? s : w;        /* whatever a masked row holds */
+                }
+                const unsigned at = (j * G + l) * V;
+                if (at < E) {
+                    if constexpr (EVEN) {
+                        store_vec<T, V>(dlogits + q * p.ld_out + at, d);
+                    } else {
+                        store_row<T, V>(dlogits + q * p.ld_out, at, E, d);
+                    }
+                }
             }
         }
-        float inv, lse;
-        row_softmax<G, C>(x, inv, lse);
-        float dot = 0.f;
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            x[k] *= inv;
-            dot = __builtin_fmaf(x[k], c[k], dot);
-        }
-        dot = group_all<G>(dot, Add());
-        const float z = b * lse;
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            const float s = __builtin_fmaf(x[k], __builtin_fmaf(a, c[k] - dot, z), d[k]);
-            d[k] = live ? s : d[k];   /* whatever grad_loss is */
-        }
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            float v[V];
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                v[k] = d[j * V + k];
-            }
-            if ((unsigned)(j * G + l) * V < E) {
-                store_row<T, V>(dlogits + t * p.ld_out, (j * G + l) * V, E, v);
-            }
-        }
+        now = next;
     }
 }
 
@@ -793,10 +952,13 @@ k_balance_grad(const T *logits, const uint8_t *mask, const int64_t *counts, cons
 /* ======================================================================== */
 struct Policy {
     uint64_t rows, cols, ld;
-    int      adv_per_row, per_sequence;
-    unsigned lanes;              /* that share a row: a power of two */
+    int      per_sequence;
+    unsigned lanes_log;          /* log2 of the lanes that share a row */
     unsigned steps;              /* vectors of a lane */
     uint64_t chunks;             /* parts of a row */
+    uint64_t whole;              /* columns in whole vectors */
+    uint64_t tail_chunk;         /* whose lane tail_lane has the others, if any */
+    unsigned tail_lane;
     float    up, down;           /* log(1 + clip_high), log(1 - clip_low) */
     float    ratio_up, ratio_down;
     float    kl_coef;
@@ -813,6 +975,12 @@ struct PolicySum {
     uint64_t tokens, rows, cut;
 };
 
+/* by the hardware's base-2 exponential (1 ulp); the scaling rounds off |x| u */
+__device__ __forceinline__ float exp_of(float x)
+{
+    return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+
 /* exp(q) - q - 1, by its series near nought, where the subtractions would
  * leave nothing (to q^10 / 10!: the rest is below 5e-9 of it there) */
 __device__ __forceinline__ float exp_less(float q)
@@ -825,57 +993,136 @@ __device__ __forceinline__ float exp_less(float q)
     s = __builtin_fmaf(s, q, 1.f / 120.f);
     s = __builtin_fmaf(s, q, 1.f / 24.f);
     s = __builtin_fmaf(s, q, 1.f / 6.f);
-    s = __builtin_fmaf(s, q, 0.5f);
-    return fabsf(q) < 0.75f ? s * q * q : expf(q) - q - 1.f;
+    s = __builtin_fmaf(s, q, 0.5f) * q * q;
+    float e = exp_of(q) - q - 1.f;
+    asm("" : "+v"(s), "+v"(e));       /* both computed: no branch around either */
+    return fabsf(q) < 0.75f ? s : e;
 }
 
-/* whether a token is cut goes by d itself, not by its rounded exponential */
-__device__ __forceinline__ bool is_cut(float a, float d, const Policy &p)
-{
-    return (a > 0.f && d > p.up) || (a < 0.f && d < p.down);
-}
+/* What an advantage makes of its tokens: d with A's sign is compared with
+ * `limit` (a token is cut goes by d itself, not by its rounded exponential;
+ * A = 0 has no limit), and `cap` is the ratio of a cut token. */
+struct Advantage {
+    float a, limit, cap;
 
-/* the operands of V tokens of a row, and which of them count */
+    __device__ __forceinline__ Advantage() = default;
+    __device__ __forceinline__ Advantage(float x, const Policy &p)
+    {
+        a     = x;
+        limit = x > 0.f ? p.up : x < 0.f ? -p.down : INFINITY;
+        cap   = x > 0.f ? p.ratio_up : p.ratio_down;
+    }
+    __device__ __forceinline__ bool cuts(float d) const
+    {
+        return __uint_as_float(__float_as_uint(d) ^ (__float_as_uint(a) & 0x80000000u)) > limit;
+    }
+};
+
+/* V neighbouring tokens of a row as they were loaded: converting them would
+ * wait for them, and the next loads would not be in flight together */
 template <typename T, int V>
 struct Tokens {
-    float logp[V], old[V], ref[V], adv[V];
-    bool  live[V];
+    T       logp[V], old[V], ref[V];
+    float   adv[V];
+    uint8_t live[V];
+};
 
-    __device__ __forceinline__ void load(const T *lp, const T *op, const T *rp,
-                                         const float *ap, const uint8_t *mp, const Policy &p,
-                                         uint64_t row, uint64_t c)
+/* what a call has of its rows: REF a reference, ROW an advantage for each row
+ * (known at compile time, since the branches would be in every token) */
+template <typename T, bool REF, bool ROW>
+struct PolicyIn {
+    const T       *logp, *old, *ref;
+    const float   *adv;
+    const uint8_t *mask;
+
+    template <int V>
+    __device__ __forceinline__ void load(uint64_t at, Tokens<T, V> &t) const
     {
-        const uint64_t at = row * p.ld;
-        load_row<T, V>(lp + at, c, p.cols, 0.f, logp);
-        load_row<T, V>(op + at, c, p.cols, 0.f, old);
-        if (rp != nullptr) {
-            load_row<T, V>(rp + at, c, p.cols, 0.f, ref);
+        load_raw<T, V>(logp + at, t.logp);
+        load_raw<T, V>(old + at, t.old);
+        if constexpr (REF) {
+            load_raw<T, V>(ref + at, t.ref);
         }
-        if (p.adv_per_row) {
-            const float a = ap[row];
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                adv[k] = a;
-            }
-        } else {
-            load_row<float, V>(ap + at, c, p.cols, 0.f, adv);
+        if constexpr (!ROW) {
+            load_raw<float, V>(adv + at, t.adv);
         }
-        if (mp == nullptr) {
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                live[k] = c + k < p.cols;
-            }
-        } else if (c + V <= p.cols) {
-            uint8_t m[V];
-            load_raw<uint8_t, V>(mp + at + c, m);
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                live[k] = m[k] != 0;
-            }
+        if (mask != nullptr) {
+            load_raw<uint8_t, V>(mask + at, t.live);
         } else {
+            __builtin_memset(t.live, 1, V);
+        }
+    }
+
+    /* one token, for the end of a row that is no whole vector */
+    __device__ __forceinline__ void load_one(uint64_t at, Tokens<T, 1> &t) const
+    {
+        t.logp[0] = logp[at];
+        t.old[0]  = old[at];
+        t.ref[0]  = REF ? ref[at] : logp[at];
+        t.adv[0]  = ROW ? 0.f : adv[at];
+        t.live[0] = mask != nullptr ? mask[at] : 1;
+    }
+};
+
+/* vectors of a lane in flight at once: 16 tokens */
+template <typename T>
+constexpr int policy_steps()
+{
+    return (int)sizeof(T);
+}
+
+/* Which part of which rows a wave does: the waves of a block lie side by side
+ * along a row's parts as far as it has them (wc = 1, 2, 4 .. of them), then
+ * along the rows; no division. */
+template <int W>
+struct PolicyWave {
+    unsigned l, per, wc_log;
+    uint64_t row_tile, chunk, tile_step, chunk_step;
+
+    __device__ __forceinline__ PolicyWave(const Policy &p)
+    {
+        const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        l      = lane & ((1u << p.lanes_log) - 1);
+        per    = 64u >> p.lanes_log;
+        wc_log = 0;
+        while ((1u << wc_log) < W && (1u << wc_log) < p.chunks) {
+            wc_log++;
+        }
+        row_tile   = ((uint64_t)blockIdx.x * (W >> wc_log)) + (wave >> wc_log);
+        chunk      = ((uint64_t)blockIdx.y << wc_log) + (wave & ((1u << wc_log) - 1));
+        tile_step  = (uint64_t)gridDim.x * (W >> wc_log);
+        chunk_step = (uint64_t)gridDim.y << wc_log;
+    }
+    __device__ __forceinline__ uint64_t row(uint64_t tile, const Policy &p) const
+    {
+        return tile * per + ((threadIdx.x & 63) >> p.lanes_log);
+    }
+};
+
+/* the sums of a lane over its tokens */
+struct PolicyAcc {
+    float    pg = 0.f, kl = 0.f;
+    unsigned tokens = 0, cut = 0;
+
+    template <bool REF, bool ROW, typename T, int V>
+    __device__ __forceinline__ void add(const Tokens<T, V> &t, const Advantage &row,
+                                        const Policy &p)
+    {
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                live[k] = c + k < p.cols && mp[at + c + k] != 0;
+        for (int k = 0; k < V; k++) {
+            const Advantage w = ROW ? row : Advantage(t.adv[k], p);
+            const float x = (float)t.logp[k], d = x - (float)t.old[k];
+            const bool on = t.live[k] != 0, is = w.cuts(d);
+            float r = exp_of(d);
+            asm("" : "+v"(r));
+            r = (is ? w.cap : r) * -w.a;
+            pg += on ? r : 0.f;
+            tokens += on;
+            cut += on & is;
+            if constexpr (REF) {
+                float e = exp_less((float)t.ref[k] - x);
+                asm("" : "+v"(e));
+                kl += on ? e : 0.f;
             }
         }
     }
@@ -883,11 +1130,12 @@ struct Tokens {
 
 /* the join of a row's parts, of the rows, and the results; by blocks that each
  * take rows b, b + gridDim.x, .. groups of them */
+template <int NT>
 __device__ __forceinline__ PolicySum policy_rows(const PolicyPart *part, const Policy &p,
                                                  int32_t *row_tokens, unsigned lanes)
 {
     PolicySum sum = {};
-    const unsigned l = threadIdx.x % lanes, per = kThreads / lanes;
+    const unsigned l = threadIdx.x % lanes, per = NT / lanes;
     for (uint64_t r = (uint64_t)blockIdx.x * per + threadIdx.x / lanes; r < p.rows;
          r += (uint64_t)gridDim.x * per) {
         double pg = 0, kl = 0;
@@ -918,15 +1166,16 @@ __device__ __forceinline__ PolicySum policy_rows(const PolicyPart *part, const P
     return sum;
 }
 
+template <int NT>
 __device__ __forceinline__ PolicySum policy_block(PolicySum s, double *lds)
 {
-    unsigned long long *n = reinterpret_cast<unsigned long long*>(lds + 4);
+    unsigned long long *n = reinterpret_cast<unsigned long long*>(lds + NT / 64);
     PolicySum t;
-    t.pg     = block_sum(s.pg, lds);
-    t.kl     = block_sum(s.kl, lds);
-    t.tokens = block_sum((unsigned long long)s.tokens, n);
-    t.rows   = block_sum((unsigned long long)s.rows, n);
-    t.cut    = block_sum((unsigned long long)s.cut, n);
+    t.pg     = block_sum<NT>(s.pg, lds);
+    t.kl     = block_sum<NT>(s.kl, lds);
+    t.tokens = block_sum<NT>((unsigned long long)s.tokens, n);
+    t.rows   = block_sum<NT>((unsigned long long)s.rows, n);
+    t.cut    = block_sum<NT>((unsigned long long)s.cut, n);
     return t;
 }
 
@@ -954,62 +1203,72 @@ __device__ __forceinline__ void policy_write(const PolicySum &s, const Policy &p
 }
 
 /* A wave does one part of 64 / lanes rows at a time: `steps` vectors of each
- * of the lanes that share the row. One block (single): it joins them too. */
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-k_policy(const T *logp, const T *old, const T *ref, const float *adv, const uint8_t *mask,
-         Policy p, PolicyPart *part, unsigned *done, int single, float *sums, int64_t *counts,
+ * of the lanes that share the row, all in flight at once. NT = kSingle: the
+ * only block, which has the parts in LDS and joins them too. */
+constexpr int kSingle      = 512;
+constexpr int kSingleParts = 1024;
+
+template <typename T, bool REF, bool ROW, int NT>
+__global__ void __launch_bounds__(NT)
+k_policy(PolicyIn<T, REF, ROW> in, Policy p, PolicyPart *part, unsigned *done, float *sums, int64_t *counts,
          int32_t *row_tokens, float *loss)
 {
-    constexpr int V = 16 / sizeof(T);
-    __shared__ double lds[8];
-    const unsigned lane = threadIdx.x & 63, l = lane % p.lanes, per = 64 / p.lanes;
-    const uint64_t tiles = (p.rows + per - 1) / per, items = tiles * p.chunks;
-    for (uint64_t it = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items;
-         it += (uint64_t)gridDim.x * 4) {
-        const uint64_t chunk = it % p.chunks;
-        const uint64_t row   = it / p.chunks * per + lane / p.lanes;
-        float pg = 0.f, kl = 0.f;
-        unsigned tokens = 0, cut = 0;
-        if (row < p.rows) {
-            const uint64_t c0 = chunk * p.steps * p.lanes * V + l * V;
-#pragma unroll 2
-            for (unsigned j = 0; j < p.steps; j++) {
-                const uint64_t c = c0 + (uint64_t)j * p.lanes * V;
-                if (c >= p.cols) {
-                    break;
-                }
-                Tokens<T, V> t;
-                t.load(logp, old, ref, adv, mask, p, row, c);
+    constexpr int V = 16 / sizeof(T), S = policy_steps<T>(), W = NT / 64;
+    constexpr bool single = NT == kSingle;
+    __shared__ double lds[2 * W];
+    __shared__ PolicyPart own[single ? kSingleParts : 1];
+    if constexpr (single) {
+        part = own;
+    }
+    const PolicyWave<W> w(p);
+    const unsigned lanes = 1u << p.lanes_log, l = w.l, cs = lanes * V;
+    for (uint64_t tile = w.row_tile; tile * w.per < p.rows; tile += w.tile_step)
+    for (uint64_t chunk = w.chunk; chunk < p.chunks; chunk += w.chunk_step) {
+        const uint64_t row   = w.row(tile, p);
+        const uint64_t c0    = chunk * p.steps * cs + l * V;
+        const uint64_t end   = row < p.rows ? p.whole : 0;
+        const uint64_t at    = row * p.ld + c0;
+        Tokens<T, V> t[S];
+        Advantage a;
+        a.a = row < p.rows && ROW ? in.adv[row] : 0.f;
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    const float d = t.logp[k] - t.old[k];
-                    const bool is = is_cut(t.adv[k], d, p);
-                    const float r = is ? (t.adv[k] > 0.f ? p.ratio_up : p.ratio_down) : expf(d);
-                    const float e = ref != nullptr ? exp_less(t.ref[k] - t.logp[k]) : 0.f;
-                    pg += t.live[k] ? -t.adv[k] * r : 0.f;
-                    kl += t.live[k] ? e : 0.f;
-                    tokens += t.live[k];
-                    cut += t.live[k] && is;
-                }
+        for (unsigned j = 0; j < S; j++) {
+            if (j < p.steps && c0 + j * cs < end) {
+                in.load(at + j * cs, t[j]);
             }
         }
-        pg     = lanes_all(pg, 1, p.lanes, Add());
-        kl     = lanes_all(kl, 1, p.lanes, Add());
-        tokens = lanes_all(tokens, 1, p.lanes, Add());
-        cut    = lanes_all(cut, 1, p.lanes, Add());
+        a = Advantage(a.a, p);
+        PolicyAcc acc;
+#pragma unroll
+        for (unsigned j = 0; j < S; j++) {
+            if (j < p.steps && c0 + j * cs < end) {
+                acc.template add<REF, ROW>(t[j], a, p);
+            }
+        }
+        /* the rest of the row, by the lane whose turn it would be */
+        if (row < p.rows && chunk == p.tail_chunk && l == p.tail_lane) {
+#pragma unroll 1
+            for (uint64_t c = p.whole; c < p.cols; c++) {
+                Tokens<T, 1> one;
+                in.load_one(row * p.ld + c, one);
+                acc.template add<REF, ROW>(one, a, p);
+            }
+        }
+        const float pg        = lanes_all(acc.pg, 1, lanes, Add());
+        const float kl        = lanes_all(acc.kl, 1, lanes, Add());
+        const unsigned tokens = lanes_all(acc.tokens, 1, lanes, Add());
+        const unsigned cut    = lanes_all(acc.cut, 1, lanes, Add());
         if (l == 0 && row < p.rows) {
             part[row * p.chunks + chunk] = {pg, kl, tokens, cut};
         }
     }
-    if (single) {
-        __threadfence();
+    if constexpr (single) {
         __syncthreads();
-        const PolicySum s = policy_block(policy_rows(part, p, row_tokens, 1), lds);
+        const PolicySum s = policy_block<NT>(policy_rows<NT>(part, p, row_tokens, 1), lds);
         if (threadIdx.x == 0) {
             policy_write(s, p, sums, counts, loss);
         }
-    } else if (blockIdx.x == 0 && threadIdx.x == 0) {
+    } else if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
         *done = 0;
     }
 }
@@ -1020,7 +1279,7 @@ k_policy_join(const PolicyPart *part, PolicySum *block, unsigned *done, Policy p
 {
     __shared__ double lds[8];
     __shared__ unsigned arrived;
-    PolicySum s = policy_block(policy_rows(part, p, row_tokens, lanes), lds);
+    PolicySum s = policy_block<kThreads>(policy_rows<kThreads>(part, p, row_tokens, lanes), lds);
     if (threadIdx.x == 0) {
         block[blockIdx.x] = s;
     }
@@ -1029,7 +1288,7 @@ k_policy_join(const PolicyPart *part, PolicySum *block, unsigned *done, Policy p
         if (threadIdx.x < gridDim.x) {
             t = block[threadIdx.x];
         }
-        t = policy_block(t, lds);
+        t = policy_block<kThreads>(t, lds);
         if (threadIdx.x == 0) {
             policy_write(t, p, sums, counts, loss);
         }
@@ -1042,51 +1301,74 @@ __global__ void k_policy_loss(const float *sums, const int64_t *counts, int per_
     policy_loss_values(sums[0], sums[1], per_sequence ? counts[1] : counts[0], kl_coef, loss);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-k_policy_grad(const T *logp, const T *old, const T *ref, const float *adv, const uint8_t *mask,
-              const int32_t *row_tokens, const int64_t *counts, const float *grad_loss, T *dlogp,
-              Policy p)
+/* the gradient of V tokens, each times its weight */
+template <bool REF, bool ROW, typename T, int V>
+__device__ __forceinline__ void policy_slope(const Tokens<T, V> &t, const Advantage &row, float w,
+                                             const Policy &p, float (&o)[V])
 {
-    constexpr int V = 16 / sizeof(T);
-    const unsigned lane = threadIdx.x & 63, l = lane % p.lanes, per = 64 / p.lanes;
-    const uint64_t tiles = (p.rows + per - 1) / per, items = tiles * p.chunks;
-    const double g   = grad_loss != nullptr ? (double)*grad_loss : 1.0;
-    const int64_t n  = p.per_sequence ? counts[1] : counts[0];
-    const double all = n > 0 ? g / (double)n : 0;
-    for (uint64_t it = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items;
-         it += (uint64_t)gridDim.x * 4) {
-        const uint64_t chunk = it % p.chunks;
-        const uint64_t row   = it / p.chunks * per + lane / p.lanes;
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+        const Advantage a = ROW ? row : Advantage(t.adv[k], p);
+        const float x = (float)t.logp[k], d = x - (float)t.old[k];
+        float r = exp_of(d);
+        asm("" : "+v"(r));
+        float g = (a.cuts(d) ? 0.f : r) * -a.a;
+        if constexpr (REF) {
+            const float q = (float)t.ref[k] - x;
+            g = __builtin_fmaf(-p.kl_coef, exp_less(q) + q, g);       /* 1 - exp(q) */
+        }
+        asm("" : "+v"(g));
+        o[k] = t.live[k] != 0 ? g * w : 0.f;
+    }
+}
+
+template <typename T, bool REF, bool ROW>
+__global__ void __launch_bounds__(kThreads)
+k_policy_grad(PolicyIn<T, REF, ROW> in, const int32_t *row_tokens, const int64_t *counts,
+              const float *grad_loss, T *dlogp, Policy p)
+{
+    constexpr int V = 16 / sizeof(T), S = policy_steps<T>();
+    const PolicyWave<kThreads / 64> w(p);
+    const unsigned l = w.l, cs = V << p.lanes_log;
+    const uint64_t end = p.whole;
+    for (uint64_t tile = w.row_tile; tile * w.per < p.rows; tile += w.tile_step)
+    for (uint64_t chunk = w.chunk; chunk < p.chunks; chunk += w.chunk_step) {
+        const uint64_t row = w.row(tile, p);
         if (row >= p.rows) {
             continue;
         }
-        float w = (float)all;
-        if (p.per_sequence) {
-            const int32_t m = row_tokens[row];
-            w = m > 0 ? (float)(all / m) : 0.f;
-        }
-        const uint64_t c0 = chunk * p.steps * p.lanes * V + l * V;
-#pragma unroll 2
-        for (unsigned j = 0; j < p.steps; j++) {
-            const uint64_t c = c0 + (uint64_t)j * p.lanes * V;
-            if (c >= p.cols) {
-                break;
-            }
-            Tokens<T, V> t;
-            t.load(logp, old, ref, adv, mask, p, row, c);
-            float o[V];
+        const uint64_t c0  = chunk * p.steps * cs + l * V;
+        const uint64_t at  = row * p.ld + c0;
+        Tokens<T, V> t[S];
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                const float d = t.logp[k] - t.old[k];
-                float x = is_cut(t.adv[k], d, p) ? 0.f : -t.adv[k] * expf(d);
-                if (ref != nullptr) {
-                    const float q = t.ref[k] - t.logp[k];
-                    x = __builtin_fmaf(-p.kl_coef, exp_less(q) + q, x);   /* 1 - exp(q) */
-                }
-                o[k] = t.live[k] ? x * w : 0.f;
+        for (unsigned j = 0; j < S; j++) {
+            if (j < p.steps && c0 + j * cs < end) {
+                in.load(at + j * cs, t[j]);
             }
-            store_row<T, V>(dlogp + row * p.ld, c, p.cols, o);
+        }
+        const Advantage a(ROW ? in.adv[row] : 0.f, p);
+        const int64_t n = p.per_sequence ? counts[1] : counts[0];
+        const double g  = grad_loss != nullptr ? (double)*grad_loss : 1.0;
+        const int m     = p.per_sequence ? row_tokens[row] : 1;
+        const float weight = n > 0 && m > 0 ? (float)(g / ((double)n * m)) : 0.f;
+#pragma unroll
+        for (unsigned j = 0; j < S; j++) {
+            if (j < p.steps && c0 + j * cs < end) {
+                float o[V];
+                policy_slope<REF, ROW>(t[j], a, weight, p, o);
+                store_vec<T, V>(dlogp + at + j * cs, o);
+            }
+        }
+        /* the rest of the row, by the lane whose turn it would be */
+        if (chunk == p.tail_chunk && l == p.tail_lane) {
+#pragma unroll 1
+            for (uint64_t c = end; c < p.cols; c++) {
+                Tokens<T, 1> one;
+                float o[1];
+                in.load_one(row * p.ld + c, one);
+                policy_slope<REF, ROW>(one, a, weight, p, o);
+                dlogp[row * p.ld + c] = (T)o[0];
+            }
         }
     }
 }
@@ -1176,6 +1458,23 @@ void with_float(int dt, F f)
     }
 }
 
+/* f(T, whether there is a reference, whether advantages are by rows) */
+template <typename F>
+void with_policy(int dt, bool ref, bool row, F f)
+{
+    with_float(dt, [&](auto t) {
+        if (ref && row) {
+            f(t, std::true_type(), std::true_type());
+        } else if (ref) {
+            f(t, std::true_type(), std::false_type());
+        } else if (row) {
+            f(t, std::false_type(), std::true_type());
+        } else {
+            f(t, std::false_type(), std::false_type());
+        }
+    });
+}
+
 /* (T of dt, R of out_dt): out_dt is dt or FLOAT32 */
 template <typename F>
 void with_pair(int dt, int out_dt, F f)
@@ -1191,14 +1490,6 @@ void with_pair(int dt, int out_dt, F f)
 }
 
 /* ---- dropout ---- */
-/* elements of a lane: a whole group of eight where 16 bytes hold it, half a
- * group where a 32-bit operand would need two loads for it */
-template <typename T, typename R>
-constexpr int drop_vec()
-{
-    return sizeof(T) == 2 && sizeof(R) == 2 ? 8 : 4;
-}
-
 /* work-items of one launch (a dispatch counts them in 32 bits) */
 constexpr uint64_t kMaxItems = (uint64_t)1 << 31;
 /* columns of a bias whose gradient one launch can join (16 to a block) */
@@ -1208,12 +1499,12 @@ template <typename T, typename R, int N>
 void launch_sum(hipStream_t st, R *dst, const SrcList &srcs, unsigned nsrc, const T *bias,
                 const R *residual, uint64_t n, uint64_t cols, const Rng &rng)
 {
-    constexpr int V = drop_vec<T, R>();
-    const uint64_t inv    = cols == 1 ? 0 : UINT64_MAX / cols + 1;
-    const uint64_t groups = div_up(n + rng.offset % V, V);
-    for (uint64_t first = 0; first < groups; first += kMaxItems) {
-        const uint64_t left = groups - first < kMaxItems ? groups - first : kMaxItems;
-        hipLaunchKernelGGL((k_sum_dropout<T, R, V, N>), dim3((unsigned)div_up(left, kThreads)),
+    constexpr uint64_t kMost = kMaxItems / 64;      /* waves of a launch */
+    const uint64_t inv   = cols == 1 ? 0 : UINT64_MAX / cols + 1;
+    const uint64_t waves = div_up(n + rng.offset % 8, kWaveElems);
+    for (uint64_t first = 0; first < waves; first += kMost) {
+        const uint64_t left = waves - first < kMost ? waves - first : kMost;
+        hipLaunchKernelGGL((k_sum_dropout<T, R, N>), dim3((unsigned)div_up(left, kThreads / 64)),
                            dim3(kThreads), 0, st, dst, srcs, nsrc, bias, residual, n, first,
                            cols, inv, rng);
     }
@@ -1234,31 +1525,31 @@ void launch_sum_n(hipStream_t st, R *dst, const SrcList &srcs, unsigned nsrc, co
     }
 }
 
-/* how the gradient with the bias' part cuts its rows: the same for every type,
- * so that the workspace goes by the sizes alone (V = 4 gives the most parts) */
+/* how the gradient with the bias' part cuts its rows */
 struct GradPlan {
     unsigned tx;                 /* lanes side by side */
-    uint64_t blocks_x, parts, chunk;
+    unsigned parts;
+    uint64_t blocks_x, chunk;
 };
 
-GradPlan grad_plan(uint64_t rows, uint64_t cols, int V)
+GradPlan grad_plan(uint64_t rows, uint64_t cols)
 {
     GradPlan g;
-    const uint64_t groups = div_up(cols, V);
+    const uint64_t groups = div_up(cols, 8);
     g.tx = 1;
-    while (g.tx < (unsigned)kThreads && g.tx < groups) {
+    while (g.tx < 64 && g.tx < groups) {
         g.tx *= 2;
     }
     g.blocks_x        = div_up(groups, g.tx);
     const uint64_t ty = kThreads / g.tx;
-    /* 1024 blocks, at most 256 parts to join, four rows a lane at least */
-    uint64_t parts = div_up(1024, g.blocks_x);
-    parts   = parts < 256 ? parts : 256;
+    /* 2048 blocks, few enough parts to join at once, four rows a lane at least */
+    uint64_t parts = div_up(2048, g.blocks_x);
+    parts   = parts < kMaxParts ? parts : kMaxParts;
     const uint64_t most = div_up(rows, ty * 4);
     parts   = parts < most ? parts : most;
     parts   = parts > 0 ? parts : 1;
     g.chunk = div_up(rows, parts);
-    g.parts = g.chunk ? div_up(rows, g.chunk) : 1;
+    g.parts = g.chunk ? (unsigned)div_up(rows, g.chunk) : 1;
     return g;
 }
 
@@ -1329,58 +1620,70 @@ ucs_status_t balance_check(const ucg_builtin_dev_balance_params_t *p, const char
     return UCS_OK;
 }
 
-/* blocks of k_balance: enough for every CU, few enough to join; a multiple of
- * 64 rows each, so that no more than one of them is short whatever G is */
+/* blocks of k_balance: one to a CU at most, and to be joined at once; 128 rows
+ * at least, which one block does by itself */
 void balance_plan(uint64_t tokens, uint64_t *blocks, uint64_t *chunk)
 {
-    constexpr uint64_t kMost = 512;
-    uint64_t c = div_up(div_up(tokens, kMost), 64) * 64;
-    c       = c ? c : 64;
+    uint64_t c = div_up(tokens, kMaxParts);
+    c       = c < 128 ? 128 : c;
     *chunk  = c;
     *blocks = tokens ? div_up(tokens, c) : 1;
 }
 
-/* f(T, G lanes to a row, NV vectors to a lane) for `experts` columns */
+/* f(G lanes to a row, NV vectors to a lane, whether the row is whole vectors)
+ * for `experts` columns */
 template <typename T, typename F>
 void with_layout(unsigned experts, F f)
 {
     constexpr unsigned V = 16 / sizeof(T);
     const unsigned groups = (unsigned)div_up(experts, V);
+    const auto even = [&](auto g, auto nv) {
+        if (experts % V == 0) {
+            f(g, nv, std::true_type());
+        } else {
+            f(g, nv, std::false_type());
+        }
+    };
     typedef std::integral_constant<int, 1> one;
     if (groups <= 1) {
-        f(one(), one());
+        even(one(), one());
     } else if (groups <= 2) {
-        f(std::integral_constant<int, 2>(), one());
+        even(std::integral_constant<int, 2>(), one());
     } else if (groups <= 4) {
-        f(std::integral_constant<int, 4>(), one());
+        even(std::integral_constant<int, 4>(), one());
     } else if (groups <= 8) {
-        f(std::integral_constant<int, 8>(), one());
+        even(std::integral_constant<int, 8>(), one());
     } else if (groups <= 16) {
-        f(std::integral_constant<int, 16>(), one());
+        even(std::integral_constant<int, 16>(), one());
     } else if (groups <= 32) {
-        f(std::integral_constant<int, 32>(), one());
+        even(std::integral_constant<int, 32>(), one());
     } else if (groups <= 64) {
-        f(std::integral_constant<int, 64>(), one());
+        even(std::integral_constant<int, 64>(), one());
     } else if (groups <= 128) {
-        f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+        even(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
     } else if constexpr (V == 4) {
-        f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+        even(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
     }
 }
 
 /* ---- policy ---- */
 constexpr unsigned kPolicyJoin = 64;      /* joining blocks at most */
 
-void policy_split(uint64_t cols, int V, Policy *p)
+void policy_split(uint64_t cols, int size, Policy *p)
 {
+    const unsigned V = 16 / size, most = size;     /* policy_steps() */
     const uint64_t groups = div_up(cols, V);
-    p->lanes = 1;
-    while (p->lanes < 64 && p->lanes < groups) {
-        p->lanes *= 2;
+    p->lanes_log = 0;
+    while (p->lanes_log < 6 && (1u << p->lanes_log) < groups) {
+        p->lanes_log++;
     }
-    const uint64_t vecs = div_up(groups, p->lanes);
-    p->steps  = (unsigned)(vecs < 4 ? (vecs ? vecs : 1) : 4);
+    const uint64_t lanes = (uint64_t)1 << p->lanes_log, vecs = div_up(groups, lanes);
+    p->steps  = (unsigned)(vecs < most ? (vecs ? vecs : 1) : most);
     p->chunks = vecs ? div_up(vecs, p->steps) : 1;
+    p->whole  = cols / V * V;
+    const uint64_t step = p->whole / (lanes * V);       /* the last vector's */
+    p->tail_chunk = p->whole < cols ? step / p->steps : UINT64_MAX;
+    p->tail_lane  = (unsigned)(p->whole / V % lanes);
 }
 
 ucs_status_t policy_check(const ucg_builtin_dev_policy_params_t *q, const char *what, Policy *p,
@@ -1406,7 +1709,6 @@ ucs_status_t policy_check(const ucg_builtin_dev_policy_params_t *q, const char *
     if (q->cols > (size_t)INT32_MAX || q->rows > ((size_t)1 << 48) || !span(q->rows, q->cols, p->ld, 4, bytes)) {
         return invalid(what, "rows x cols does not fit");
     }
-    p->adv_per_row  = q->adv_per_row;
     p->per_sequence = q->per_sequence;
     p->up           = (float)log1p(q->clip_high);
     p->down         = (float)log1p(-q->clip_low);
@@ -1414,15 +1716,22 @@ ucs_status_t policy_check(const ucg_builtin_dev_policy_params_t *q, const char *
     p->ratio_down   = (float)(1 - q->clip_low);
     p->kl_coef      = (float)q->kl_coef;
     p->kl_coef64    = q->kl_coef;
-    policy_split(q->cols, 16 / (int)size_of(q->dt), p);
+    policy_split(q->cols, (int)size_of(q->dt), p);
     return UCS_OK;
 }
 
-unsigned policy_grid(const Policy &p)
+/* blocks of W waves as PolicyWave lays them out */
+dim3 policy_grid(const Policy &p, uint64_t W)
 {
-    const uint64_t items = div_up(p.rows, 64 / p.lanes) * p.chunks;
-    const uint64_t b     = div_up(items, 4);
-    return (unsigned)(b < (1u << 20) ? (b ? b : 1) : (1u << 20));
+    uint64_t wc = 1;
+    while (wc < W && wc < p.chunks) {
+        wc *= 2;
+    }
+    const uint64_t x = div_up(div_up(p.rows, (uint64_t)64 >> p.lanes_log), W / wc);
+    const uint64_t y = div_up(p.chunks, wc);
+    const uint64_t most = 1u << 20;    /* the kernels go on from there in a loop */
+    const uint64_t gy = y < 1024 ? y : 1024, gx = x ? x : 1;
+    return dim3((unsigned)(gx < most / gy ? gx : most / gy), (unsigned)gy);
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -1492,16 +1801,11 @@ ucs_status_t ucg_builtin_dev_sum_dropout(ucg_builtin_dev_ctx_t *ctx,
 
 size_t ucg_builtin_dev_sum_dropout_grad_workspace(size_t rows, size_t cols)
 {
-    size_t most = 0;
     if (cols == 0 || cols > kMaxBias) {
         return 0;
     }
-    for (int v : {4, 8}) {
-        const GradPlan g   = grad_plan(rows, cols, v);
-        const size_t bytes = g.parts > 1 ? g.parts * cols * sizeof(float) : 0;
-        most = bytes > most ? bytes : most;
-    }
-    return round16(most);
+    const GradPlan g = grad_plan(rows, cols);
+    return g.parts > 1 ? round16(g.parts * cols * sizeof(float)) : 0;
 }
 
 ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
@@ -1561,16 +1865,15 @@ ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
             dev_ctx_count(ctx, 1, 0);
             return;
         }
-        constexpr int V     = drop_vec<T, R>();
-        const GradPlan plan = grad_plan(rows, cols, V);
+        const GradPlan plan = grad_plan(rows, cols);
         float *out          = plan.parts > 1 ? static_cast<float*>(workspace) : dbias;
-        const dim3 grid((unsigned)plan.blocks_x, (unsigned)plan.parts);
-        if (cols % V == 0 && rng.offset % V == 0) {
-            hipLaunchKernelGGL((k_dropout_grad<R, T, V, true>), grid, dim3(kThreads), 0, stream,
-                               d, g, out, rows, cols, plan.tx, plan.chunk, rng);
+        const dim3 grid((unsigned)plan.blocks_x, plan.parts);
+        if (cols % 8 == 0 && rng.offset % 8 == 0) {
+            hipLaunchKernelGGL((k_dropout_grad<R, T, true>), grid, dim3(kThreads), 0, stream, d,
+                               g, out, rows, cols, plan.tx, plan.chunk, rng);
         } else {
-            hipLaunchKernelGGL((k_dropout_grad<R, T, V, false>), grid, dim3(kThreads), 0, stream,
-                               d, g, out, rows, cols, plan.tx, plan.chunk, rng);
+            hipLaunchKernelGGL((k_dropout_grad<R, T, false>), grid, dim3(kThreads), 0, stream, d,
+                               g, out, rows, cols, plan.tx, plan.chunk, rng);
         }
         if (plan.parts > 1) {
             hipLaunchKernelGGL(k_join_bias, dim3((unsigned)div_up(cols, 16)), dim3(kThreads), 0,
@@ -1637,16 +1940,19 @@ ucs_status_t ucg_builtin_dev_balance(ucg_builtin_dev_ctx_t *ctx,
     int64_t *direct    = blocks > 1 ? nullptr : counts;
     with_float(params->dt, [&](auto t) {
         typedef decltype(t) T;
-        with_layout<T>(b.experts, [&](auto g, auto nv) {
+        with_layout<T>(b.experts, [&](auto g, auto nv, auto even) {
             constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+            constexpr bool EVEN = decltype(even)::value;
             if (is == 4) {
-                hipLaunchKernelGGL((k_balance<T, int32_t, G, NV>), dim3((unsigned)blocks),
-                                   dim3(kThreads), 0, stream, static_cast<const T*>(logits),
+                hipLaunchKernelGGL((k_balance<T, int32_t, G, NV, EVEN>), dim3((unsigned)blocks),
+                                   dim3(kBalanceThreads), 0, stream,
+                                   static_cast<const T*>(logits),
                                    static_cast<const int32_t*>(index), mask, b, part, direct,
                                    sums, loss);
             } else {
-                hipLaunchKernelGGL((k_balance<T, int64_t, G, NV>), dim3((unsigned)blocks),
-                                   dim3(kThreads), 0, stream, static_cast<const T*>(logits),
+                hipLaunchKernelGGL((k_balance<T, int64_t, G, NV, EVEN>), dim3((unsigned)blocks),
+                                   dim3(kBalanceThreads), 0, stream,
+                                   static_cast<const T*>(logits),
                                    static_cast<const int64_t*>(index), mask, b, part, direct,
                                    sums, loss);
             }
@@ -1731,11 +2037,12 @@ ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
     hipStream_t stream = stream_of(ctx);
     with_float(params->dt, [&](auto t) {
         typedef decltype(t) T;
-        with_layout<T>(b.experts, [&](auto g, auto nv) {
+        with_layout<T>(b.experts, [&](auto g, auto nv, auto even) {
             constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
-            const uint64_t want = div_up(b.tokens, 4 * (64 / G));
-            const unsigned grid = (unsigned)(want < 2048 ? want : 2048);
-            hipLaunchKernelGGL((k_balance_grad<T, G, NV>), dim3(grid), dim3(kThreads), 0, stream,
+            constexpr bool EVEN = decltype(even)::value;
+            const uint64_t want = div_up(b.tokens, 4 * (64 / G) * (NV == 1 ? 2 : 1));
+            const unsigned grid = (unsigned)(want < 1024 ? want : 1024);
+            hipLaunchKernelGGL((k_balance_grad<T, G, NV, EVEN>), dim3(grid), dim3(kThreads), 0, stream,
                                static_cast<const T*>(logits), mask, counts,
                                static_cast<const T*>(base), grad_loss, static_cast<T*>(dlogits),
                                b);
@@ -1750,9 +2057,9 @@ ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
 size_t ucg_builtin_dev_policy_workspace(size_t rows, size_t cols)
 {
     size_t most = 1;
-    for (int v : {4, 8}) {
+    for (int size : {2, 4}) {
         Policy p;
-        policy_split(cols, v, &p);
+        policy_split(cols, size, &p);
         most = p.chunks > most ? p.chunks : most;
     }
     return round16(rows * most * sizeof(PolicyPart)) + round16(kPolicyJoin * sizeof(PolicySum)) +
@@ -1799,16 +2106,21 @@ ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
     OnDevice dev(dev_ctx_device(ctx));
     HIP_TRY(dev.err);
     hipStream_t stream = stream_of(ctx);
-    unsigned grid      = policy_grid(p);
+    const dim3 grid    = policy_grid(p, kThreads / 64);
     /* one block does a few parts by itself: a second launch costs more */
-    const int single = grid <= 4 && p.rows <= (uint64_t)kThreads;
-    grid = single ? 1 : grid;
-    with_float(params->dt, [&](auto t) {
+    const bool single = grid.x * grid.y <= 4 && p.rows * p.chunks <= (uint64_t)kSingleParts;
+    with_policy(params->dt, ref != nullptr, params->adv_per_row != 0, [&](auto t, auto rf, auto rw) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((k_policy<T>), dim3(grid), dim3(kThreads), 0, stream,
-                           static_cast<const T*>(logp), static_cast<const T*>(old),
-                           static_cast<const T*>(ref), adv, mask, p, part, done, single, sums,
-                           counts, row_tokens, loss);
+        constexpr bool REF = decltype(rf)::value, ROW = decltype(rw)::value;
+        const PolicyIn<T, REF, ROW> in = {static_cast<const T*>(logp), static_cast<const T*>(old),
+                                          static_cast<const T*>(ref), adv, mask};
+        if (single) {
+            hipLaunchKernelGGL((k_policy<T, REF, ROW, kSingle>), dim3(1), dim3(kSingle), 0, stream,
+                               in, p, part, done, sums, counts, row_tokens, loss);
+        } else {
+            hipLaunchKernelGGL((k_policy<T, REF, ROW, kThreads>), grid, dim3(kThreads), 0, stream,
+                               in, p, part, done, sums, counts, row_tokens, loss);
+        }
     });
     if (!single) {
         unsigned lanes = 1;
@@ -1881,7 +2193,7 @@ ucs_status_t ucg_builtin_dev_policy_grad(ucg_builtin_dev_ctx_t *ctx,
     if ((dlogp != logp && overlap(dlogp, nb, logp, nb)) ||
         (dlogp != old && overlap(dlogp, nb, old, nb)) ||
         (ref != nullptr && dlogp != ref && overlap(dlogp, nb, ref, nb)) ||
-        overlap(dlogp, nb, adv, p.adv_per_row ? p.rows * 4 : bytes) ||
+        overlap(dlogp, nb, adv, params->adv_per_row ? p.rows * 4 : bytes) ||
         (mask != nullptr && overlap(dlogp, nb, mask, bytes / 4)) ||
         (row_tokens != nullptr && overlap(dlogp, nb, row_tokens, p.rows * 4)) ||
         (grad_loss != nullptr && overlap(dlogp, nb, grad_loss, 4)) ||
@@ -1896,12 +2208,14 @@ ucs_status_t ucg_builtin_dev_policy_grad(ucg_builtin_dev_ctx_t *ctx,
     }
     OnDevice dev(dev_ctx_device(ctx));
     HIP_TRY(dev.err);
-    with_float(params->dt, [&](auto t) {
+    with_policy(params->dt, ref != nullptr, params->adv_per_row != 0, [&](auto t, auto rf, auto rw) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((k_policy_grad<T>), dim3(policy_grid(p)), dim3(kThreads), 0,
-                           stream_of(ctx), static_cast<const T*>(logp),
-                           static_cast<const T*>(old), static_cast<const T*>(ref), adv, mask,
-                           row_tokens, counts, grad_loss, static_cast<T*>(dlogp), p);
+        constexpr bool REF = decltype(rf)::value, ROW = decltype(rw)::value;
+        const PolicyIn<T, REF, ROW> in = {static_cast<const T*>(logp), static_cast<const T*>(old),
+                                          static_cast<const T*>(ref), adv, mask};
+        hipLaunchKernelGGL((k_policy_grad<T, REF, ROW>), policy_grid(p, kThreads / 64),
+                           dim3(kThreads), 0, stream_of(ctx), in, row_tokens, counts, grad_loss,
+                           static_cast<T*>(dlogp), p);
     });
     HIP_TRY(hipGetLastError());
     dev_ctx_count(ctx, 1, 0);
