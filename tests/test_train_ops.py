@@ -3,7 +3,6 @@ refusals and layouts on the CPU, numerics on the GPU against 64-bit numpy
 (oracle/train_ref.py). Every bound below is counted from the operations a
 value goes through, u = 2^-24 for each in fp32, and half a step of the output's
 type for its one rounding."""
-import ctypes
 import os
 import subprocess
 
@@ -85,24 +84,29 @@ def test_reference_gradients_are_those_of_differences():
 
 
 def test_parameter_structs_match_the_header(tmp_path):
-    """sizeof and every offset of the ctypes structures are the compiler's."""
-    pairs = (("ucg_builtin_dev_dropout_params_t", _lib.DropoutParams),
-             ("ucg_builtin_dev_balance_params_t", _lib.BalanceParams),
-             ("ucg_builtin_dev_policy_params_t", _lib.PolicyParams))
+    """What Python packs is what a C program reads in the header's structs,
+    field by field."""
+    pairs = (("dropout", _lib.DROPOUT_FIELDS, _lib.DropoutParams,
+              (10, 9, 3 << 40, 5 << 41, 0.125, 2 ** 64 - 7, 2 ** 63 + 9, 77, PTR)),
+             ("balance", _lib.BALANCE_FIELDS, _lib.BalanceParams,
+              (8, 6, 1 << 50, 2, 3, 4, 5 << 40, 6, 0.5, -0.25)),
+             ("policy", _lib.POLICY_FIELDS, _lib.PolicyParams,
+              (9, 1, 0, 1 << 33, 2 << 34, 3 << 35, 0.25, 4.5, -8.0)))
     lines, want = [], []
-    for name, s in pairs:
-        lines.append(f'printf("%zu\\n", sizeof({name}));')
-        want.append(ctypes.sizeof(s))
-        for f, _ in s._fields_:
-            lines.append(f'printf("%zu\\n", offsetof({name}, {f}));')
-            want.append(getattr(s, f).offset)
+    for name, fields, pack, values in pairs:
+        lines.append(f'{{ ucg_builtin_dev_{name}_params_t q; if (fread(&q, sizeof(q), 1, stdin) != 1) return 1;')
+        lines += [f'printf("%.17g\\n", (double)(uintptr_t)q.{f});' if f == "rng" else
+                  f'printf("%.17g\\n", (double)q.{f});' for f in fields]
+        lines.append("}")
+        want.append((pack(*values), values))
+    lines.append("return getchar() == EOF ? 0 : 2;")
     src = tmp_path / "p.c"
     src.write_text('#include <stdio.h>\n#include "ucg_builtin_dev.h"\nint main(void) {\n' +
-                   "\n".join(lines) + "\nreturn 0; }\n")
+                   "\n".join(lines) + "\n}\n")
     exe = str(tmp_path / "p")
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe], check=True)
-    got = subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()
-    assert [int(x) for x in got] == want
+    p = subprocess.run([exe], input=b"".join(w for w, _ in want), check=True, capture_output=True)
+    assert [float(x) for x in p.stdout.split()] == [float(x) for _, v in want for x in v]
 
 
 def refused(fn, status, why, *args):
@@ -113,12 +117,12 @@ def refused(fn, status, why, *args):
 
 
 def srcs_of(*ptrs):
-    return (ctypes.c_void_p * len(ptrs))(*ptrs)
+    return _lib.addresses(ptrs)
 
 
 def test_sum_dropout_refusals():
     def P(dt="float32", out="float32", rows=4, cols=8, p=0.1, offset=0, rng=None):
-        return _lib.DropoutParams(DT[dt], DT[out], rows, cols, p, 1, 2, offset, rng)
+        return _lib.DropoutParams(DT[dt], DT[out], rows, cols, p, 1, 2, offset, rng or 0)
     f, s = "ucg_builtin_dev_sum_dropout", srcs_of(PTR)
 
     def bad(why, q, dst=2 * PTR, srcs=s, n=1, bias=None, res=None, status=INVALID):
@@ -156,7 +160,7 @@ def test_sum_dropout_grad_refusals():
     f = "ucg_builtin_dev_sum_dropout_grad"
 
     def P(dt="float32", out="float32", rows=4000, cols=8, p=0.1):
-        return _lib.DropoutParams(DT[dt], DT[out], rows, cols, p, 1, 2, 0, None)
+        return _lib.DropoutParams(DT[dt], DT[out], rows, cols, p, 1, 2, 0, 0)
     need = xucg_amd.DevContext.sum_dropout_grad_workspace(4000, 8)
     assert need > 0 and need % 16 == 0
     assert xucg_amd.DevContext.sum_dropout_grad_workspace(0, 8) == 0
@@ -905,7 +909,8 @@ def test_torch_tensors_and_captured_graphs(in_child):
             ("rng", lambda: ctx.sum_dropout("float32", out, [r], rows, cols, 0.1, 1, rng=state[:1])),
             ("index", lambda: ctx.balance("float32", logits, index.int(), rows, e, k, counts, sums, workspace=ws[1])),
             ("counts", lambda: ctx.balance("float32", logits, index, rows, e, k, counts[:-1], sums, workspace=ws[1])),
-            ("logits", lambda: ctx.balance("float32", logits, index, rows, e, k, counts, sums, ld=e + 1)),
+            ("logits", lambda: ctx.balance("float32", logits, index, rows, e, k, counts, sums, ld=e + 1,
+                                           workspace=ws[1])),
             ("adv", lambda: ctx.policy("float32", lp, old, adv, rows, cols, ps, pc, workspace=ws[2])),
             ("workspace", lambda: ctx.policy("float32", lp, old, adv, rows, cols, ps, pc, adv_per_row=True,
                                              workspace=ws[2].cpu()))):

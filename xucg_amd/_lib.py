@@ -9,6 +9,7 @@ or fails to load, this module raises and the caller fails loudly.
 """
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(HERE, "lib")
@@ -54,28 +55,22 @@ class DevCtxParams(ctypes.Structure):
                 ("zcopy_bytes", ctypes.c_size_t), ("completion", ctypes.c_int)]
 
 
-class DropoutParams(ctypes.Structure):
-    """ucg_builtin_dev_dropout_params_t"""
-    _fields_ = [("dt", ctypes.c_int), ("out_dt", ctypes.c_int), ("rows", ctypes.c_size_t),
-                ("cols", ctypes.c_size_t), ("p", ctypes.c_double), ("seed", ctypes.c_uint64),
-                ("tag", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("rng", ctypes.c_void_p)]
+# The parameter structs of the training-step operators. A call packs one with
+# struct (a ctypes structure costs four times as long to fill, and these calls
+# may be shorter on the GPU than on the host); the fields, in order, are
+DROPOUT_FIELDS = ("dt", "out_dt", "rows", "cols", "p", "seed", "tag", "offset", "rng")
+BALANCE_FIELDS = ("dt", "index_dt", "tokens", "experts", "topk", "ld", "ld_index", "ld_out",
+                  "balance_coef", "z_coef")
+POLICY_FIELDS = ("dt", "adv_per_row", "per_sequence", "rows", "cols", "ld", "clip_low",
+                 "clip_high", "kl_coef")
+DropoutParams = struct.Struct("@iiNNdQQQP").pack       # ucg_builtin_dev_dropout_params_t
+BalanceParams = struct.Struct("@iiNNNNNNdd").pack      # ucg_builtin_dev_balance_params_t
+PolicyParams = struct.Struct("@iiiNNNddd").pack        # ucg_builtin_dev_policy_params_t
 
 
-class BalanceParams(ctypes.Structure):
-    """ucg_builtin_dev_balance_params_t"""
-    _fields_ = [("dt", ctypes.c_int), ("index_dt", ctypes.c_int), ("tokens", ctypes.c_size_t),
-                ("experts", ctypes.c_size_t), ("topk", ctypes.c_size_t), ("ld", ctypes.c_size_t),
-                ("ld_index", ctypes.c_size_t), ("ld_out", ctypes.c_size_t),
-                ("balance_coef", ctypes.c_double), ("z_coef", ctypes.c_double)]
-
-
-class PolicyParams(ctypes.Structure):
-    """ucg_builtin_dev_policy_params_t"""
-    _fields_ = [("dt", ctypes.c_int), ("adv_per_row", ctypes.c_int),
-                ("per_sequence", ctypes.c_int), ("rows", ctypes.c_size_t),
-                ("cols", ctypes.c_size_t), ("ld", ctypes.c_size_t),
-                ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double),
-                ("kl_coef", ctypes.c_double)]
+def addresses(ptrs):
+    """a C array of pointers (None: NULL)"""
+    return struct.pack(f"{len(ptrs)}P", *(p or 0 for p in ptrs))
 
 
 ZCOPY_NEVER = (1 << 64) - 1   # UCG_BUILTIN_DEV_ZCOPY_NEVER
@@ -110,22 +105,21 @@ DEV_API = {
     "ucg_builtin_dev_gather_multi": (_st, [_vp, _vp, ctypes.POINTER(_vp), _u, _sz]),
     "ucg_builtin_dev_copy_multi": (_st, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp), _u,
                                          _sz]),
-    "ucg_builtin_dev_sum_dropout": (_st, [_vp, ctypes.POINTER(DropoutParams), _vp,
-                                          ctypes.POINTER(_vp), _u, _vp, _vp]),
+    "ucg_builtin_dev_sum_dropout": (_st, [_vp, _vp, _vp, _vp, _u, _vp, _vp]),
     "ucg_builtin_dev_sum_dropout_grad_workspace": (_sz, [_sz, _sz]),
-    "ucg_builtin_dev_sum_dropout_grad": (_st, [_vp, ctypes.POINTER(DropoutParams), _vp, _vp,
+    "ucg_builtin_dev_sum_dropout_grad": (_st, [_vp, _vp, _vp, _vp,
                                                _vp, _vp, _sz]),
     "ucg_builtin_dev_balance_workspace": (_sz, [_sz, _sz]),
-    "ucg_builtin_dev_balance": (_st, [_vp, ctypes.POINTER(BalanceParams), _vp, _vp, _vp, _vp,
+    "ucg_builtin_dev_balance": (_st, [_vp, _vp, _vp, _vp, _vp, _vp,
                                       _vp, _vp, _vp, _sz]),
-    "ucg_builtin_dev_balance_loss": (_st, [_vp, ctypes.POINTER(BalanceParams), _vp, _vp, _vp]),
-    "ucg_builtin_dev_balance_grad": (_st, [_vp, ctypes.POINTER(BalanceParams), _vp, _vp, _vp,
+    "ucg_builtin_dev_balance_loss": (_st, [_vp, _vp, _vp, _vp, _vp]),
+    "ucg_builtin_dev_balance_grad": (_st, [_vp, _vp, _vp, _vp, _vp,
                                            _vp, _vp, _vp]),
     "ucg_builtin_dev_policy_workspace": (_sz, [_sz, _sz]),
-    "ucg_builtin_dev_policy": (_st, [_vp, ctypes.POINTER(PolicyParams), _vp, _vp, _vp, _vp, _vp,
+    "ucg_builtin_dev_policy": (_st, [_vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      _vp, _vp, _vp, _vp, _vp, _sz]),
-    "ucg_builtin_dev_policy_loss": (_st, [_vp, ctypes.POINTER(PolicyParams), _vp, _vp, _vp]),
-    "ucg_builtin_dev_policy_grad": (_st, [_vp, ctypes.POINTER(PolicyParams), _vp, _vp, _vp, _vp,
+    "ucg_builtin_dev_policy_loss": (_st, [_vp, _vp, _vp, _vp, _vp]),
+    "ucg_builtin_dev_policy_grad": (_st, [_vp, _vp, _vp, _vp, _vp, _vp,
                                           _vp, _vp, _vp, _vp, _vp]),
     "ucg_builtin_dev_combine_host": (_st, [_vp, _int, _int, _vp, _vp, _sz]),
     "ucg_builtin_dev_stage_begin": (_st, [_vp, _vp, _sz]),

@@ -37,17 +37,15 @@ def _ptr(x):
 _DT = {name: i for i, name in enumerate(_lib.DTYPES)}
 
 
-class _TorchNames(dict):
-    """torch dtype -> its name here; filled on first sight, torch not imported"""
-    def __missing__(self, dtype):
-        name = self[dtype] = str(dtype).rpartition(".")[2]
-        return name
-
-    def get(self, dtype, default=None):
-        return self[dtype]
+_TORCH = {}     # name -> torch dtype, filled by the tensors that come (torch not imported)
 
 
-_TORCH_NAME = _TorchNames()
+def _is_dtype(dtype, name):
+    """whether a torch dtype is the type `name` (a uint8 mask may be bool)"""
+    known = str(dtype).rpartition(".")[2]
+    if known == name:
+        _TORCH[name] = dtype
+    return known == name or (name == "uint8" and known == "bool")
 
 
 def _name(dt):
@@ -251,49 +249,47 @@ class DevContext:
         return _lib.dev().ucg_builtin_dev_copy_multi(self.handle, da, sa, n, nbytes)
 
     # -- operators of a training step beside the combine -------------------
-    def _operands(self, *specs):
-        """Addresses of (name, buffer, dtype, shape, row step) operands. A torch
-        tensor is held to them: the type, this context's device, as many
-        elements, and rows `row step` apart whose elements are neighbours."""
-        out = []
-        for name, x, dt, shape, ld in specs:
-            if x is None or isinstance(x, int) or not hasattr(x, "data_ptr"):
-                out.append(_ptr(x))
-                continue
-            if _TORCH_NAME.get(x.dtype) != dt and not (
-                    dt == "uint8" and _TORCH_NAME.get(x.dtype) == "bool"):
-                raise ValueError(f"{name}: {dt} wanted, got {x.dtype}")
-            if x.device.type != "cuda" or x.device.index != self.device:
-                raise ValueError(f"{name}: a tensor on cuda:{self.device} wanted, got one on "
-                                 f"{x.device}")
-            want = 1
-            for n in shape:
-                want *= n
-            if x.numel() < want if ld is None else x.numel() != want:
-                raise ValueError(f"{name}: {tuple(shape)} wanted, got {tuple(x.shape)}")
-            if not x.is_contiguous() or (ld or shape[-1]) != shape[-1]:
-                if not (ld and want and x.dim() == 2 and tuple(x.shape) == tuple(shape) and
-                        (shape[1] == 1 or x.stride(1) == 1) and
-                        (shape[0] == 1 or x.stride(0) == ld)):
-                    raise ValueError(f"{name}: strides {x.stride()} where rows of neighbours, "
-                                     f"{ld or shape[-1]} apart, are wanted")
-            out.append(x.data_ptr())
-        return out
+    def _at(self, name, x, dt, n, row=0, step=0):
+        """The address of operand `name`. A torch tensor is held to what the
+        call reads or writes there: the type, this context's device, n
+        elements without gaps - or in rows of `row` that lie `step` apart."""
+        if x is None or x.__class__ is int:
+            return x
+        try:
+            dtype = x.dtype
+            address = x.data_ptr()
+        except AttributeError:
+            return _ptr(x)
+        if dtype is not _TORCH.get(dt) and not _is_dtype(dtype, dt):
+            raise ValueError(f"{name}: {dt} wanted, got {dtype}")
+        if x.get_device() != self.device:
+            raise ValueError(f"{name}: a tensor on cuda:{self.device} wanted, got {x.device}")
+        if x.numel() != n:
+            raise ValueError(f"{name}: {n} elements wanted, got {tuple(x.shape)}")
+        if step == row:
+            if not x.is_contiguous():
+                raise ValueError(f"{name}: a contiguous tensor wanted, got strides {x.stride()}")
+        elif n and (x.dim() != 2 or x.shape[1] != row or (row > 1 and x.stride(1) != 1) or
+                    (n > row and x.stride(0) != step)):
+            raise ValueError(f"{name}: rows of {row}, {step} apart, wanted, got "
+                             f"{tuple(x.shape)} with strides {x.stride()}")
+        return address
 
     def sum_dropout(self, dt, dst, srcs, rows, cols, p, seed, tag=0, offset=0, bias=None,
                     residual=None, out_dt=None, rng=None):
         """dst = residual + dropout(sum of srcs + bias), the mask a function of
         (seed, tag, offset + element) that is never stored
-        (ucg_builtin_dev_sum_dropout)."""
-        dt, out_dt, shape = _name(dt), _name(dt if out_dt is None else out_dt), (rows, cols)
-        dst, bias, residual, rng, *srcs = self._operands(
-            ("dst", dst, out_dt, shape, cols), ("bias", bias, dt, (cols,), cols),
-            ("residual", residual, out_dt, shape, cols), ("rng", rng, "int64", (2,), 2),
-            *(("srcs", s, dt, shape, cols) for s in srcs))
-        q = _lib.DropoutParams(_DT[dt], _DT[out_dt], rows, cols, p, seed, tag, offset, rng)
-        check(_lib.dev().ucg_builtin_dev_sum_dropout(
-            self.handle, q, dst, (ctypes.c_void_p * len(srcs))(*srcs), len(srcs), bias,
-            residual), "ucg_builtin_dev_sum_dropout")
+        (ucg_builtin_dev_sum_dropout). rng: device memory holding {seed, tag}."""
+        dt, at, n = _name(dt), self._at, rows * cols
+        out_dt = dt if out_dt is None else _name(out_dt)
+        srcs = [at("srcs", s, dt, n) for s in srcs]
+        q = _lib.DropoutParams(_DT[dt], _DT[out_dt], rows, cols, p, seed, tag, offset,
+                               at("rng", rng, "int64", 2) or 0)
+        st = _lib.dev().ucg_builtin_dev_sum_dropout(
+            self.handle, q, at("dst", dst, out_dt, n), _lib.addresses(srcs), len(srcs),
+            at("bias", bias, dt, cols), at("residual", residual, out_dt, n))
+        if st:
+            check(st, "ucg_builtin_dev_sum_dropout")
 
     @staticmethod
     def sum_dropout_grad_workspace(rows, cols):
@@ -304,15 +300,16 @@ class DevContext:
                          grad_dt=None, workspace=None, rng=None):
         """dsrc = the gradient of every source of sum_dropout, dbias (cols
         floats) = the bias' (ucg_builtin_dev_sum_dropout_grad)."""
-        dt, grad_dt, shape = _name(dt), _name(dt if grad_dt is None else grad_dt), (rows, cols)
-        dsrc, grad, dbias, rng = self._operands(
-            ("dsrc", dsrc, dt, shape, cols), ("grad", grad, grad_dt, shape, cols),
-            ("dbias", dbias, "float32", (cols,), cols), ("rng", rng, "int64", (2,), 2))
-        q = _lib.DropoutParams(_DT[dt], _DT[grad_dt], rows, cols, p, seed, tag, offset, rng)
+        dt, at, n = _name(dt), self._at, rows * cols
+        grad_dt = dt if grad_dt is None else _name(grad_dt)
+        q = _lib.DropoutParams(_DT[dt], _DT[grad_dt], rows, cols, p, seed, tag, offset,
+                               at("rng", rng, "int64", 2) or 0)
         ws, nbytes = self._workspace(workspace, self.sum_dropout_grad_workspace, rows, cols)
-        check(_lib.dev().ucg_builtin_dev_sum_dropout_grad(self.handle, q, dsrc, grad, dbias, ws,
-                                                          nbytes),
-              "ucg_builtin_dev_sum_dropout_grad")
+        st = _lib.dev().ucg_builtin_dev_sum_dropout_grad(
+            self.handle, q, at("dsrc", dsrc, dt, n), at("grad", grad, grad_dt, n),
+            at("dbias", dbias, "float32", cols), ws, nbytes)
+        if st:
+            check(st, "ucg_builtin_dev_sum_dropout_grad")
 
     def _workspace(self, workspace, need, *sizes):
         """A workspace's address and bytes. An address alone is taken to hold
@@ -322,10 +319,9 @@ class DevContext:
         if isinstance(workspace, int):
             return workspace, need(*sizes)
         if hasattr(workspace, "data_ptr"):
-            if workspace.device.type != "cuda" or workspace.device.index != self.device or \
-                    not workspace.is_contiguous():
+            if workspace.get_device() != self.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace: a contiguous tensor on cuda:{self.device} wanted")
-            return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            return workspace.data_ptr(), workspace.nbytes
         return workspace.ptr, workspace.nbytes
 
     @staticmethod
@@ -340,49 +336,45 @@ class DevContext:
         (experts + 1 float32: probability of each expert, squared log sum exp)
         of this member's tokens: what the group adds up
         (ucg_builtin_dev_balance). loss: 3 floats, for a group of one."""
-        dt, index_dt = _name(dt), _name(index_dt)
-        logits, index, mask, counts, sums, loss = self._operands(
-            ("logits", logits, dt, (tokens, experts), ld or experts),
-            ("index", index, index_dt, (tokens, topk), ld_index or topk),
-            ("mask", mask, "uint8", (tokens,), tokens),
-            ("counts", counts, "int64", (experts + 1,), None),
-            ("sums", sums, "float32", (experts + 1,), None),
-            ("loss", loss, "float32", (3,), None))
+        dt, index_dt, at = _name(dt), _name(index_dt), self._at
         q = _lib.BalanceParams(_DT[dt], _DT[index_dt], tokens, experts, topk, ld, ld_index, 0,
                                balance_coef, z_coef)
         ws, nbytes = self._workspace(workspace, self.balance_workspace, tokens, experts)
-        check(_lib.dev().ucg_builtin_dev_balance(self.handle, q, logits, index, mask, counts,
-                                                 sums, loss, ws, nbytes),
-              "ucg_builtin_dev_balance")
+        st = _lib.dev().ucg_builtin_dev_balance(
+            self.handle, q,
+            at("logits", logits, dt, tokens * experts, experts, ld or experts),
+            at("index", index, index_dt, tokens * topk, topk, ld_index or topk),
+            at("mask", mask, "uint8", tokens), at("counts", counts, "int64", experts + 1),
+            at("sums", sums, "float32", experts + 1), at("loss", loss, "float32", 3), ws, nbytes)
+        if st:
+            check(st, "ucg_builtin_dev_balance")
 
     def balance_loss(self, counts, sums, experts, topk, loss, balance_coef=0.0, z_coef=0.0):
         """loss (3 floats: whole, balance part, z part) from the group's counts
         and sums (ucg_builtin_dev_balance_loss)."""
-        counts, sums, loss = self._operands(("counts", counts, "int64", (experts + 1,), None),
-                                            ("sums", sums, "float32", (experts + 1,), None),
-                                            ("loss", loss, "float32", (3,), None))
+        at = self._at
         q = _lib.BalanceParams(_DT["float32"], _DT["int64"], 0, experts, topk, 0, 0, 0,
                                balance_coef, z_coef)
-        check(_lib.dev().ucg_builtin_dev_balance_loss(self.handle, q, counts, sums, loss),
-              "ucg_builtin_dev_balance_loss")
+        check(_lib.dev().ucg_builtin_dev_balance_loss(
+            self.handle, q, at("counts", counts, "int64", experts + 1),
+            at("sums", sums, "float32", experts + 1), at("loss", loss, "float32", 3)),
+            "ucg_builtin_dev_balance_loss")
 
     def balance_grad(self, dt, dlogits, logits, tokens, experts, topk, counts, mask=None,
                      base=None, grad_loss=None, balance_coef=0.0, z_coef=0.0, ld=0, ld_out=0):
         """dlogits = base + grad_loss * the loss' gradient, with the group's
         counts (ucg_builtin_dev_balance_grad)."""
-        dt = _name(dt)
-        dlogits, logits, mask, counts, base, grad_loss = self._operands(
-            ("dlogits", dlogits, dt, (tokens, experts), ld_out or experts),
-            ("logits", logits, dt, (tokens, experts), ld or experts),
-            ("mask", mask, "uint8", (tokens,), tokens),
-            ("counts", counts, "int64", (experts + 1,), None),
-            ("base", base, dt, (tokens, experts), ld_out or experts),
-            ("grad_loss", grad_loss, "float32", (1,), None))
+        dt, at, n = _name(dt), self._at, tokens * experts
         q = _lib.BalanceParams(_DT[dt], _DT["int64"], tokens, experts, topk, ld, 0, ld_out,
                                balance_coef, z_coef)
-        check(_lib.dev().ucg_builtin_dev_balance_grad(self.handle, q, logits, mask, counts, base,
-                                                      grad_loss, dlogits),
-              "ucg_builtin_dev_balance_grad")
+        st = _lib.dev().ucg_builtin_dev_balance_grad(
+            self.handle, q, at("logits", logits, dt, n, experts, ld or experts),
+            at("mask", mask, "uint8", tokens), at("counts", counts, "int64", experts + 1),
+            at("base", base, dt, n, experts, ld_out or experts),
+            at("grad_loss", grad_loss, "float32", 1),
+            at("dlogits", dlogits, dt, n, experts, ld_out or experts))
+        if st:
+            check(st, "ucg_builtin_dev_balance_grad")
 
     @staticmethod
     def policy_workspace(rows, cols):
@@ -396,53 +388,48 @@ class DevContext:
         tokens, rows that have one, cut tokens) of this member's answers: what
         the group adds up (ucg_builtin_dev_policy). loss: 3 floats, for a group
         of one."""
-        dt, shape, step = _name(dt), (rows, cols), ld or cols
-        logp, old, ref, adv, mask, sums, counts, row_tokens, loss = self._operands(
-            ("logp", logp, dt, shape, step), ("old", old, dt, shape, step),
-            ("ref", ref, dt, shape, step),
-            ("adv", adv, "float32", (rows,) if adv_per_row else shape,
-             rows if adv_per_row else step),
-            ("mask", mask, "uint8", shape, step), ("sums", sums, "float32", (2,), None),
-            ("counts", counts, "int64", (3,), None),
-            ("row_tokens", row_tokens, "int32", (rows,), None),
-            ("loss", loss, "float32", (3,), None))
+        dt, at, n, step = _name(dt), self._at, rows * cols, ld or cols
         q = _lib.PolicyParams(_DT[dt], adv_per_row, per_sequence, rows, cols, ld, clip_low,
                               clip_high, kl_coef)
         ws, nbytes = self._workspace(workspace, self.policy_workspace, rows, cols)
-        check(_lib.dev().ucg_builtin_dev_policy(self.handle, q, logp, old, ref, adv, mask, sums,
-                                                counts, row_tokens, loss, ws, nbytes),
-              "ucg_builtin_dev_policy")
+        st = _lib.dev().ucg_builtin_dev_policy(
+            self.handle, q, at("logp", logp, dt, n, cols, step), at("old", old, dt, n, cols, step),
+            at("ref", ref, dt, n, cols, step),
+            at("adv", adv, "float32", rows) if adv_per_row else
+            at("adv", adv, "float32", n, cols, step),
+            at("mask", mask, "uint8", n, cols, step), at("sums", sums, "float32", 2),
+            at("counts", counts, "int64", 3), at("row_tokens", row_tokens, "int32", rows),
+            at("loss", loss, "float32", 3), ws, nbytes)
+        if st:
+            check(st, "ucg_builtin_dev_policy")
 
     def policy_loss(self, sums, counts, loss, per_sequence=False, kl_coef=0.0):
         """loss (3 floats: whole, policy mean, KL mean) from the group's sums
         and counts (ucg_builtin_dev_policy_loss)."""
-        sums, counts, loss = self._operands(("sums", sums, "float32", (2,), None),
-                                            ("counts", counts, "int64", (3,), None),
-                                            ("loss", loss, "float32", (3,), None))
+        at = self._at
         q = _lib.PolicyParams(_DT["float32"], 0, per_sequence, 0, 0, 0, 0.0, 0.0, kl_coef)
-        check(_lib.dev().ucg_builtin_dev_policy_loss(self.handle, q, sums, counts, loss),
-              "ucg_builtin_dev_policy_loss")
+        check(_lib.dev().ucg_builtin_dev_policy_loss(
+            self.handle, q, at("sums", sums, "float32", 2), at("counts", counts, "int64", 3),
+            at("loss", loss, "float32", 3)), "ucg_builtin_dev_policy_loss")
 
     def policy_grad(self, dt, dlogp, logp, old, adv, rows, cols, counts, ref=None, mask=None,
                     row_tokens=None, adv_per_row=False, per_sequence=False, clip_low=0.2,
                     clip_high=0.2, kl_coef=0.0, grad_loss=None, ld=0):
         """dlogp = grad_loss * the loss' gradient, with the group's counts
         (ucg_builtin_dev_policy_grad)."""
-        dt, shape, step = _name(dt), (rows, cols), ld or cols
-        dlogp, logp, old, ref, adv, mask, row_tokens, counts, grad_loss = self._operands(
-            ("dlogp", dlogp, dt, shape, step), ("logp", logp, dt, shape, step),
-            ("old", old, dt, shape, step), ("ref", ref, dt, shape, step),
-            ("adv", adv, "float32", (rows,) if adv_per_row else shape,
-             rows if adv_per_row else step),
-            ("mask", mask, "uint8", shape, step),
-            ("row_tokens", row_tokens, "int32", (rows,), None),
-            ("counts", counts, "int64", (3,), None),
-            ("grad_loss", grad_loss, "float32", (1,), None))
+        dt, at, n, step = _name(dt), self._at, rows * cols, ld or cols
         q = _lib.PolicyParams(_DT[dt], adv_per_row, per_sequence, rows, cols, ld, clip_low,
                               clip_high, kl_coef)
-        check(_lib.dev().ucg_builtin_dev_policy_grad(self.handle, q, logp, old, ref, adv, mask,
-                                                     row_tokens, counts, grad_loss, dlogp),
-              "ucg_builtin_dev_policy_grad")
+        st = _lib.dev().ucg_builtin_dev_policy_grad(
+            self.handle, q, at("logp", logp, dt, n, cols, step), at("old", old, dt, n, cols, step),
+            at("ref", ref, dt, n, cols, step),
+            at("adv", adv, "float32", rows) if adv_per_row else
+            at("adv", adv, "float32", n, cols, step),
+            at("mask", mask, "uint8", n, cols, step),
+            at("row_tokens", row_tokens, "int32", rows), at("counts", counts, "int64", 3),
+            at("grad_loss", grad_loss, "float32", 1), at("dlogp", dlogp, dt, n, cols, step))
+        if st:
+            check(st, "ucg_builtin_dev_policy_grad")
 
     def combine_host(self, op, dt, dst_host, src_host, count):
         return _lib.dev().ucg_builtin_dev_combine_host(self.handle, op_index(op),
