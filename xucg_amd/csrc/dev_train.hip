@@ -253,6 +253,21 @@ __device__ __forceinline__ void draw(uint64_t at, uint64_t tag, uint64_t seed, u
     }
 }
 
+/* An even lane has computed a group of the first of two tiles, its odd neighbour
+ * one of the second; both get their half (the lower, the upper) of each. */
+__device__ __forceinline__ void share_groups(const uint32_t (&w)[4], bool odd, uint32_t *first,
+                                             uint32_t *second)
+{
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t mine = odd ? w[2 + k] : w[k];
+        const uint32_t give = odd ? w[k] : w[2 + k];
+        const uint32_t got  = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xB1, 0xf, 0xf, true);
+        first[k]  = odd ? got : mine;
+        second[k] = odd ? mine : got;
+    }
+}
+
 /* 16-bit number k of the words */
 __device__ __forceinline__ bool kept(const uint32_t *u, int k, uint32_t threshold)
 {
@@ -294,14 +309,15 @@ constexpr int kWaveElems = 512;
  * with e <= 1).
  */
 template <typename T, typename R, int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(64)
 k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *residual,
-              uint64_t n, uint64_t first, uint64_t cols, uint64_t inv, Rng rng)
+              uint64_t n, uint64_t first, int map, uint64_t cols, uint64_t inv, Rng rng)
 {
     constexpr int V = sizeof(T) == 2 && sizeof(R) == 2 ? 8 : 4, TL = 8 / V, NN = N ? N : 1;
     const unsigned phase = (unsigned)(rng.offset % 8);
-    const unsigned lane  = threadIdx.x & 63;
-    const uint64_t wave  = first + (uint64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const unsigned lane  = threadIdx.x;
+    const uint64_t wave  = first + (map ? ucgdev::xcd_tile<ucgdev::kXcdChunk>(blockIdx.x, gridDim.x)
+                                        : blockIdx.x);
     const int64_t  begin = (int64_t)(wave * kWaveElems) - phase;     /* the wave's first */
     if (begin >= (int64_t)n) {
         return;
@@ -340,18 +356,8 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
                 u[0][k] = w[k];
             }
         } else {
-            const bool odd = lane & 1;
-            philox(group + (odd ? 32 : 0) + lane / 2, tag, seed, w);
-            /* an even lane keeps the lower half of its group, an odd one the upper */
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t mine = odd ? w[2 + k] : w[k];
-                const uint32_t give = odd ? w[k] : w[2 + k];
-                const uint32_t got  = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0xB1, 0xf, 0xf,
-                                                                         true);
-                u[0][k]      = odd ? got : mine;
-                u[TL - 1][k] = odd ? mine : got;
-            }
+            philox(group + (lane & 1 ? 32 : 0) + lane / 2, tag, seed, w);
+            share_groups(w, lane & 1, u[0], u[TL - 1]);
         }
     }
 
@@ -442,68 +448,89 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
 
 /*
  * The gradient with the bias' part: a lane keeps eight columns over the rows of
- * its chunk, tx lanes side by side and kThreads / tx rows at once, and the
- * block's rows are joined in LDS. Four rows are loaded while the four before
- * them are computed. A row may start anywhere in a group of eight (ALIGNED 0:
- * the columns or the offset are no multiple of eight): then a lane's numbers
- * come from two groups.
+ * its chunk, tx lanes side by side and kThreads / tx rows at once, four rows in
+ * flight, and the block's rows are joined in LDS. With 16-bit types the eight
+ * are neighbours. A 32-bit operand would take two loads 32 bytes apart in each
+ * lane for that, so its lanes have four columns in each of two tiles and share
+ * groups as in k_sum_dropout (SPLIT). A row may start anywhere in a group of
+ * eight (ALIGNED 0: the columns or the offset are no multiple of eight): then
+ * the eight are neighbours whose numbers come from two groups.
  */
 template <typename R, typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t cols,
-               unsigned tx, uint64_t chunk, Rng rng)
+               unsigned tx, Rng rng)
 {
-    constexpr int V = 8, U = 4;
-    __shared__ float lds[kThreads * V];
+    constexpr bool SPLIT = ALIGNED && (sizeof(R) == 4 || sizeof(T) == 4);
+    constexpr int U = 4, TL = SPLIT ? 2 : 1, V = 8 / TL;
+    __shared__ float lds[kThreads * 8];
     const unsigned x  = threadIdx.x % tx, y = threadIdx.x / tx, ty = kThreads / tx;
-    const uint64_t c  = ((uint64_t)blockIdx.x * tx + x) * V;
-    const uint64_t r0 = (uint64_t)blockIdx.y * chunk;
-    const uint64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
+    const uint64_t c0 = (uint64_t)blockIdx.x * tx * 8;          /* the block's first column */
+    const uint64_t c  = c0 + x * V, tile = (uint64_t)tx * V;
+    /* part b of P takes rows b * ty + y, then P * ty further on: at any time the
+     * parts read neighbouring rows, and not rows a power of two apart */
+    const uint64_t step = (uint64_t)gridDim.y * ty;
     uint64_t seed, tag;
     rng_state(rng, seed, tag);
-    float sum[V] = {};
-    if (c + V <= cols && r0 + y < r1) {
-        const uint64_t last = r1 - 1;
-        R g[U][V];
+    float sum[8] = {};
+    bool has[TL];                     /* whether a tile's vector lies in the row */
 #pragma unroll
-        for (int j = 0; j < U; j++) {
-            const uint64_t q = r0 + y + (uint64_t)j * ty;
-            load_raw<R, V>(grad + (q < r1 ? q : last) * cols + c, g[j]);
-        }
-        for (uint64_t row = r0 + y; row < r1; row += (uint64_t)U * ty) {
-            R next[U][V];
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const uint64_t q = row + (uint64_t)(U + j) * ty;
-                load_raw<R, V>(grad + (q < r1 ? q : last) * cols + c, next[j]);
-            }
+    for (int j = 0; j < TL; j++) {
+        has[j] = c + j * tile + V <= cols;
+    }
+    /* SPLIT: cols is a multiple of eight, so a lane and its neighbour are both
+     * in or both out; the lanes of a row take part as long as one tile does */
+    if (has[0]) {
+        for (uint64_t row = (uint64_t)blockIdx.y * ty + y; row < rows; row += U * step) {
+            R g[U][TL][V];
 #pragma unroll
             for (int j = 0; j < U; j++) {
-                const uint64_t q = row + (uint64_t)j * ty;
-                if (q < r1) {
-                    uint32_t u[4] = {};
-                    if (rng.threshold != 0) {
-                        draw<ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
-                    }
-                    float d[V];
+                const uint64_t q = row + j * step;
 #pragma unroll
-                    for (int k = 0; k < V; k++) {
-                        d[k] = kept(u, k, rng.threshold) ? (float)g[j][k] * rng.scale : 0.f;
-                        sum[k] += d[k];
-                    }
-                    store_vec<T, V>(dsrc + q * cols + c, d);
+                for (int h = 0; h < TL; h++) {
+                    load_raw<R, V>(grad + (q < rows ? q : row) * cols + c + (has[h] ? h * tile : 0),
+                                   g[j][h]);
                 }
             }
-            __builtin_memcpy(g, next, sizeof(g));
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                const uint64_t q = row + j * step;
+                if (q < rows) {
+                    uint32_t u[8 / 2] = {};
+                    const uint64_t at = rng.offset + q * cols;
+                    if (rng.threshold != 0) {
+                        if constexpr (SPLIT) {
+                            uint32_t w[4];
+                            philox((at + c0 + (x & 1 ? tile : 0)) / 8 + x / 2, tag, seed, w);
+                            share_groups(w, x & 1, u, u + 2);
+                        } else {
+                            draw<ALIGNED>(at + c, tag, seed, u);
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < TL; h++) {
+                        float d[V];
+#pragma unroll
+                        for (int k = 0; k < V; k++) {
+                            d[k] = kept(u, h * V + k, rng.threshold)
+                                       ? (float)g[j][h][k] * rng.scale : 0.f;
+                            sum[h * V + k] += d[k];
+                        }
+                        if (has[h]) {
+                            store_vec<T, V>(dsrc + q * cols + c + h * tile, d);
+                        }
+                    }
+                }
+            }
         }
-    } else if (c < cols) {
-        for (uint64_t q = r0 + y; q < r1; q += ty) {
+    } else if (c < cols) {            /* not SPLIT: there a vector is in or out */
+        for (uint64_t q = (uint64_t)blockIdx.y * ty + y; q < rows; q += step) {
             uint32_t u[4] = {};
             if (rng.threshold != 0) {
                 draw<ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
             }
 #pragma unroll
-            for (int k = 0; k < V; k++) {
+            for (int k = 0; k < 8; k++) {
                 if (c + k < cols) {
                     const float d = kept(u, k, rng.threshold)
                                         ? (float)grad[q * cols + c + k] * rng.scale : 0.f;
@@ -514,19 +541,18 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
         }
     }
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-        lds[threadIdx.x * V + k] = sum[k];
+    for (int k = 0; k < 8; k++) {
+        lds[y * tx * 8 + (k / V) * tile + x * V + k % V] = sum[k];
     }
     __syncthreads();
-    /* column j of the block's tx * V: its rows y = 0, 1, .. in order */
-    for (unsigned j = threadIdx.x; j < tx * V; j += kThreads) {
-        const uint64_t at = (uint64_t)blockIdx.x * tx * V + j;
-        if (at < cols) {
+    /* column j of the block's tx * 8: its rows y = 0, 1, .. in order */
+    for (unsigned j = threadIdx.x; j < tx * 8; j += kThreads) {
+        if (c0 + j < cols) {
             float s = 0.f;
             for (unsigned q = 0; q < ty; q++) {
-                s += lds[q * tx * V + j];
+                s += lds[q * tx * 8 + j];
             }
-            dbias[(uint64_t)blockIdx.y * cols + at] = s;
+            dbias[(uint64_t)blockIdx.y * cols + c0 + j] = s;
         }
     }
 }
@@ -665,11 +691,11 @@ __device__ __forceinline__ void load_logits(const T *row, unsigned c, unsigned E
     }
 }
 
-/* rows of a lane group in flight at once: what 16 to 32 registers of values hold */
+/* rows of a lane group in flight at once, beside as many computed */
 template <int NV>
 constexpr int rows_at_once()
 {
-    return NV == 1 ? 4 : NV == 2 ? 2 : 1;
+    return NV == 1 ? 2 : 1;
 }
 
 constexpr int kBalanceThreads = 1024;  /* 16 waves: one block to a CU */
@@ -1128,24 +1154,36 @@ struct PolicyAcc {
     }
 };
 
-/* the join of a row's parts, of the rows, and the results; by blocks that each
- * take rows b, b + gridDim.x, .. groups of them */
+/* The join of a row's parts by `lanes` lanes, eight parts of each in flight at
+ * once, and the thread's sum over its rows; block b of the grid takes rows
+ * b * NT / lanes, .. */
 template <int NT>
 __device__ __forceinline__ PolicySum policy_rows(const PolicyPart *part, const Policy &p,
                                                  int32_t *row_tokens, unsigned lanes)
 {
+    constexpr int U = 8;
     PolicySum sum = {};
     const unsigned l = threadIdx.x % lanes, per = NT / lanes;
     for (uint64_t r = (uint64_t)blockIdx.x * per + threadIdx.x / lanes; r < p.rows;
          r += (uint64_t)gridDim.x * per) {
         double pg = 0, kl = 0;
         unsigned long long tokens = 0, cut = 0;
-        for (uint64_t w = l; w < p.chunks; w += lanes) {
-            const PolicyPart &x = part[r * p.chunks + w];
-            pg += x.pg;
-            kl += x.kl;
-            tokens += x.tokens;
-            cut += x.cut;
+        for (uint64_t w = l; w < p.chunks; w += (uint64_t)U * lanes) {
+            PolicyPart x[U];
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                const uint64_t q = w + (uint64_t)j * lanes;
+                x[j] = part[r * p.chunks + (q < p.chunks ? q : w)];
+            }
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                if (w + (uint64_t)j * lanes < p.chunks) {
+                    pg += x[j].pg;
+                    kl += x[j].kl;
+                    tokens += x[j].tokens;
+                    cut += x[j].cut;
+                }
+            }
         }
         pg     = lanes_all(pg, 1, lanes, Add());
         kl     = lanes_all(kl, 1, lanes, Add());
@@ -1495,6 +1533,13 @@ constexpr uint64_t kMaxItems = (uint64_t)1 << 31;
 /* columns of a bias whose gradient one launch can join (16 to a block) */
 constexpr uint64_t kMaxBias = (uint64_t)1 << 27;
 
+/* whether the waves' parts of an operand begin inside a 128-byte line */
+template <typename T>
+bool off_line(const void *p, uint64_t phase)
+{
+    return ((uintptr_t)p - phase * sizeof(T)) % 128 != 0;
+}
+
 template <typename T, typename R, int N>
 void launch_sum(hipStream_t st, R *dst, const SrcList &srcs, unsigned nsrc, const T *bias,
                 const R *residual, uint64_t n, uint64_t cols, const Rng &rng)
@@ -1502,11 +1547,15 @@ void launch_sum(hipStream_t st, R *dst, const SrcList &srcs, unsigned nsrc, cons
     constexpr uint64_t kMost = kMaxItems / 64;      /* waves of a launch */
     const uint64_t inv   = cols == 1 ? 0 : UINT64_MAX / cols + 1;
     const uint64_t waves = div_up(n + rng.offset % 8, kWaveElems);
+    const uint64_t phase = rng.offset % 8;
+    bool map = off_line<R>(dst, phase) || (residual != nullptr && off_line<R>(residual, phase));
+    for (unsigned m = 0; m < nsrc; m++) {
+        map = map || off_line<T>(srcs.p[m], phase);
+    }
     for (uint64_t first = 0; first < waves; first += kMost) {
         const uint64_t left = waves - first < kMost ? waves - first : kMost;
-        hipLaunchKernelGGL((k_sum_dropout<T, R, N>), dim3((unsigned)div_up(left, kThreads / 64)),
-                           dim3(kThreads), 0, st, dst, srcs, nsrc, bias, residual, n, first,
-                           cols, inv, rng);
+        hipLaunchKernelGGL((k_sum_dropout<T, R, N>), dim3((unsigned)left), dim3(64), 0, st, dst,
+                           srcs, nsrc, bias, residual, n, first, (int)map, cols, inv, rng);
     }
 }
 
@@ -1529,27 +1578,27 @@ void launch_sum_n(hipStream_t st, R *dst, const SrcList &srcs, unsigned nsrc, co
 struct GradPlan {
     unsigned tx;                 /* lanes side by side */
     unsigned parts;
-    uint64_t blocks_x, chunk;
+    uint64_t blocks_x;
 };
 
 GradPlan grad_plan(uint64_t rows, uint64_t cols)
 {
     GradPlan g;
     const uint64_t groups = div_up(cols, 8);
-    g.tx = 1;
+    g.tx = 2;                    /* neighbours share groups */
     while (g.tx < 64 && g.tx < groups) {
         g.tx *= 2;
     }
     g.blocks_x        = div_up(groups, g.tx);
     const uint64_t ty = kThreads / g.tx;
-    /* 2048 blocks, few enough parts to join at once, four rows a lane at least */
-    uint64_t parts = div_up(2048, g.blocks_x);
+    /* 1024 blocks (2048 write twice the partials: 28.9 against 27.2 us for
+     * 8192 x 4096 bf16), few enough parts to join at once, four rows a lane at
+     * least */
+    uint64_t parts = div_up(1024, g.blocks_x);
     parts   = parts < kMaxParts ? parts : kMaxParts;
     const uint64_t most = div_up(rows, ty * 4);
     parts   = parts < most ? parts : most;
-    parts   = parts > 0 ? parts : 1;
-    g.chunk = div_up(rows, parts);
-    g.parts = g.chunk ? (unsigned)div_up(rows, g.chunk) : 1;
+    g.parts = parts > 0 ? (unsigned)parts : 1;
     return g;
 }
 
@@ -1620,14 +1669,22 @@ ucs_status_t balance_check(const ucg_builtin_dev_balance_params_t *p, const char
     return UCS_OK;
 }
 
-/* blocks of k_balance: one to a CU at most, and to be joined at once; 128 rows
- * at least, which one block does by itself */
-void balance_plan(uint64_t tokens, uint64_t *blocks, uint64_t *chunk)
+/* Blocks of k_balance: one to a CU at most, and to be joined at once. One block
+ * does up to 32768 logits by itself, which takes less than a second launch (200
+ * tokens of 8 experts 4.5 against 8.5 us, 300 of 64 6.2 against 10.2, 4000 of 8 the
+ * same); beyond, 128 rows a block at least (more rows in fewer blocks took
+ * longer: 4096 of 64 12.1 against 10.3 us at 512 rows). */
+void balance_plan(uint64_t tokens, uint64_t experts, uint64_t *blocks, uint64_t *chunk)
 {
-    uint64_t c = div_up(tokens, kMaxParts);
-    c       = c < 128 ? 128 : c;
-    *chunk  = c;
-    *blocks = tokens ? div_up(tokens, c) : 1;
+    constexpr uint64_t kAlone = 32768;
+    if (tokens <= kAlone / experts) {
+        *chunk  = tokens;
+        *blocks = 1;
+        return;
+    }
+    const uint64_t c = div_up(tokens, kMaxParts);
+    *chunk  = c < 128 ? 128 : c;
+    *blocks = div_up(tokens, *chunk);
 }
 
 /* f(G lanes to a row, NV vectors to a lane, whether the row is whole vectors)
@@ -1870,10 +1927,10 @@ ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
         const dim3 grid((unsigned)plan.blocks_x, plan.parts);
         if (cols % 8 == 0 && rng.offset % 8 == 0) {
             hipLaunchKernelGGL((k_dropout_grad<R, T, true>), grid, dim3(kThreads), 0, stream, d,
-                               g, out, rows, cols, plan.tx, plan.chunk, rng);
+                               g, out, rows, cols, plan.tx, rng);
         } else {
             hipLaunchKernelGGL((k_dropout_grad<R, T, false>), grid, dim3(kThreads), 0, stream, d,
-                               g, out, rows, cols, plan.tx, plan.chunk, rng);
+                               g, out, rows, cols, plan.tx, rng);
         }
         if (plan.parts > 1) {
             hipLaunchKernelGGL(k_join_bias, dim3((unsigned)div_up(cols, 16)), dim3(kThreads), 0,
@@ -1889,7 +1946,10 @@ ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
 size_t ucg_builtin_dev_balance_workspace(size_t tokens, size_t experts)
 {
     uint64_t blocks, chunk;
-    balance_plan(tokens, &blocks, &chunk);
+    if (experts == 0) {
+        return 0;
+    }
+    balance_plan(tokens, experts, &blocks, &chunk);
     return blocks > 1 ? round16(blocks * (experts + 1) * 8 + 4) : 0;
 }
 
@@ -1927,7 +1987,7 @@ ucs_status_t ucg_builtin_dev_balance(ucg_builtin_dev_ctx_t *ctx,
         return invalid(what, "ctx is NULL");
     }
     uint64_t blocks;
-    balance_plan(b.tokens, &blocks, &b.chunk);
+    balance_plan(b.tokens, b.experts, &blocks, &b.chunk);
     BalancePart part = {};
     if (blocks > 1) {
         part.sums   = static_cast<float*>(workspace);
@@ -2123,8 +2183,8 @@ ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
         }
     });
     if (!single) {
-        unsigned lanes = 1;
-        while (lanes < 64 && lanes < p.chunks) {
+        unsigned lanes = 1;               /* with eight parts each */
+        while (lanes < 64 && lanes * 8 < p.chunks) {
             lanes *= 2;
         }
         const uint64_t want = div_up(p.rows * lanes, kThreads);
