@@ -384,7 +384,7 @@ def test_sum_dropout_drops_what_is_not_finite(dev_ctx, dt):
     x = np.ones((rows, cols))
     x[~keep] = np.nan
     x[0] = np.where(keep[0], 1, np.inf)
-    a, out = Arr(dev_ctx, R.to_storage(x, dt)), Arr(dev_ctx, R.to_storage(x * 0 + 7, dt))
+    a, out = Arr(dev_ctx, R.to_storage(x, dt)), Arr(dev_ctx, R.to_storage(np.full((rows, cols), 7.0), dt))
     dev_ctx.sum_dropout(dt, out.ptr, [a.ptr], rows, cols, p, 1, tag=2)
     dev_ctx.sync()
     assert (val(out.get(), dt) == np.where(keep, 2.0, 0.0)).all()
@@ -742,6 +742,122 @@ def test_policy_clip_goes_by_the_difference(dev_ctx):
         dev_ctx.sync()
         assert c.get().tolist() == [8, 1, sum(cut)]
         assert ((g.get()[0] == 0) == (np.array(cut, bool) | (adv[0] == 0))).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+def test_policy_far_references(dev_ctx, dt):
+    """A reference that is -inf, the type's lowest value or merely far: the KL
+    gradient is 1 - exp(q), to -1 and without a NaN."""
+    low = {"float32": -3.4028234663852886e38, "bfloat16": -3.3895313892515355e38, "float16": -65504.0}[dt]
+    ref = R.to_storage(np.array([[-np.inf, low, -60000.0, -30.0, -0.75, -0.5, 0.0, 0.75, 3.0]]), dt)
+    zero = R.to_storage(np.zeros((1, 9)), dt)
+    la, ra, aa, d = Arr(dev_ctx, zero), Arr(dev_ctx, ref), Arr(dev_ctx, np.zeros((1, 9), np.float32)), \
+        Arr(dev_ctx, zero)
+    c = Arr(dev_ctx, np.array([9, 1, 0], np.int64))
+    dev_ctx.policy_grad(dt, d.ptr, la.ptr, la.ptr, aa.ptr, 1, 9, c.ptr, ref=ra.ptr, kl_coef=1.0)
+    dev_ctx.sync()
+    want = -np.expm1(R.from_storage(ref, dt)) / 9
+    off = np.abs(R.from_storage(d.get(), dt) - want)
+    # exp2 (2 u), its scaling (3 |q| u, |q| < 4 where the exponential is not nothing), the
+    # difference (u), the weight's and the type's rounding
+    assert (off <= (20 * U * np.maximum(1, np.exp(R.from_storage(ref, dt))) / 9 +
+                    R.EPS[dt] * 1.01 * np.abs(want) + R.LEAST[dt])).all()
+
+
+@gpu
+def test_places_beyond_32_bits(dev_ctx):
+    """More than 2^32 elements in a call, and row steps of more than 2^31: the
+    far end gets what a call on it alone gets."""
+    rows, cols = 65537, 65536 + 8
+    n = rows * cols
+    src, out = dev_ctx.alloc(2 * n), dev_ctx.alloc(2 * n)
+    dev_ctx.fill("bfloat16", "round", 1, src, n)
+    dev_ctx.sum_dropout("bfloat16", out.ptr, [src.ptr], rows, cols, 0.5, 3, offset=5)
+    tail = dev_ctx.alloc(2 * 3 * cols)
+    at = (rows - 3) * cols
+    dev_ctx.sum_dropout("bfloat16", tail.ptr, [src.ptr + 2 * at], 3, cols, 0.5, 3, offset=5 + at)
+    dev_ctx.sync()
+    got = out.download(np.uint16, 3 * cols, 2 * at)
+    assert (got == tail.download(np.uint16, 3 * cols)).all()
+    keep = R.keep(3, 0, 5 + at, 3 * cols, 0.5)
+    assert (got[~keep] == 0).all() and (got[keep] != 0).all()
+    dev_ctx.sum_dropout_grad("bfloat16", out.ptr, src.ptr, rows, cols, 0.5, 3, offset=5)
+    dev_ctx.sync()
+    assert (out.download(np.uint16, 3 * cols, 2 * at) == got).all()
+    # rows 2^31 + 64 elements apart, in the same memory
+    ld, size = (1 << 31) + 64, 100
+    assert 2 * ld + size <= n
+    rng = np.random.default_rng(6)
+    x = R.to_storage(rng.normal(size=(3, size)), "bfloat16")
+    near, far = Arr(dev_ctx, x), Arr(dev_ctx, np.zeros_like(x))
+    for r in range(2):
+        src.upload(x[r], 2 * r * ld)
+    c = [Arr(dev_ctx, np.zeros(size + 1, np.int64)) for _ in range(2)]
+    s = [Arr(dev_ctx, np.zeros(size + 1, np.float32)) for _ in range(2)]
+    i = Arr(dev_ctx, np.zeros((2, 1), np.int32))
+    for k, (p, step) in enumerate(((near.ptr, 0), (src.ptr, ld))):
+        dev_ctx.balance("bfloat16", p, i.ptr, 2, size, 1, c[k].ptr, s[k].ptr, index_dt="int32", ld=step)
+    dev_ctx.balance_grad("bfloat16", out.ptr, src.ptr, 2, size, 1, c[0].ptr, balance_coef=1.0, ld=ld, ld_out=ld)
+    dev_ctx.balance_grad("bfloat16", far.ptr, near.ptr, 2, size, 1, c[0].ptr, balance_coef=1.0)
+    dev_ctx.sync()
+    assert (c[0].get() == c[1].get()).all() and (s[0].get() == s[1].get()).all()
+    for r in range(2):
+        assert (out.download(np.uint16, size, 2 * r * ld) == far.get()[r]).all()
+    adv = Arr(dev_ctx, np.ones(2, np.float32))
+    pc, ps = Arr(dev_ctx, np.zeros(3, np.int64)), [Arr(dev_ctx, np.zeros(2, np.float32)) for _ in range(2)]
+    ws = dev_ctx.alloc(dev_ctx.policy_workspace(2, size))
+    for k, (p, step) in enumerate(((near.ptr, 0), (src.ptr, ld))):
+        dev_ctx.policy("bfloat16", p, p, adv.ptr, 2, size, ps[k].ptr, pc.ptr, ref=p, adv_per_row=True, ld=step,
+                       workspace=ws)
+    dev_ctx.policy_grad("bfloat16", out.ptr, src.ptr, src.ptr, adv.ptr, 2, size, pc.ptr, adv_per_row=True, ld=ld)
+    dev_ctx.policy_grad("bfloat16", far.ptr, near.ptr, near.ptr, adv.ptr, 2, size, pc.ptr, adv_per_row=True)
+    dev_ctx.sync()
+    assert (ps[0].get() == ps[1].get()).all() and pc.get().tolist() == [2 * size, 2, 0]
+    for r in range(2):
+        assert (out.download(np.uint16, size, 2 * r * ld) == far.get()[r]).all()
+    for b in (src, out):
+        b.free()
+
+
+@gpu
+def test_two_contexts_at_once(dev_ctx):
+    """Two threads, a context, a stream and workspaces each: the results of one
+    after the other."""
+    import threading
+    rng = np.random.default_rng(12)
+    rows, cols = 3000, 257
+    x = [rng.normal(size=(rows, cols)).astype(np.float32) for _ in range(2)]
+    idx = [np.argsort(-v, 1)[:, :2].astype(np.int64) for v in x]
+
+    def work(ctx, k, out):
+        a, i = Arr(ctx, x[k]), Arr(ctx, idx[k])
+        d, db = Arr(ctx, x[k] * 0), Arr(ctx, np.zeros(cols, np.float32))
+        c, s = Arr(ctx, np.zeros(cols + 1, np.int64)), Arr(ctx, np.zeros(cols + 1, np.float32))
+        loss, pc, ps = (Arr(ctx, np.zeros(n, t)) for n, t in ((3, np.float32), (3, np.int64), (2, np.float32)))
+        ws = [ctx.alloc(max(16, n)) for n in (ctx.sum_dropout_grad_workspace(rows, cols),
+                                              ctx.balance_workspace(rows, cols), ctx.policy_workspace(rows, cols))]
+        for _ in range(20):
+            ctx.sum_dropout_grad("float32", d.ptr, a.ptr, rows, cols, 0.1, k, dbias=db.ptr, workspace=ws[0])
+            ctx.balance("float32", a.ptr, i.ptr, rows, cols, 2, c.ptr, s.ptr, loss=loss.ptr, balance_coef=1.0,
+                        workspace=ws[1])
+            ctx.policy("float32", a.ptr, d.ptr, a.ptr, rows, cols, ps.ptr, pc.ptr, workspace=ws[2])
+        ctx.sync()
+        out[k] = [v.get() for v in (d, db, c, s, loss, pc, ps)]
+    alone, both = {}, {}
+    for k in range(2):
+        work(dev_ctx, k, alone)
+    ctxs = [xucg_amd.DevContext(device=0) for _ in range(2)]
+    ts = [threading.Thread(target=work, args=(ctxs[k], k, both)) for k in range(2)]
+    for th in ts:
+        th.start()
+    for th in ts:
+        th.join()
+    for k in range(2):
+        for v, w in zip(alone[k], both[k]):
+            assert (v.view(np.uint8) == w.view(np.uint8)).all()
+    for c in ctxs:
+        c.close()
 
 
 # ---- together ----------------------------------------------------------------------

@@ -305,9 +305,10 @@ constexpr int kWaveElems = 512;
  * operand a 16-byte vector is four elements: the wave has two tiles of 64
  * vectors, even lanes compute a group of the first tile and odd lanes one of
  * the second, and each hands its neighbour the half that it needs. (Half a
- * group used by each lane instead costs a second Philox: 234 against 2xx us.)
- * N operands (0: nsrc of them, one by one) and the residual are all in flight
- * before the numbers are computed.
+ * group used by each lane instead costs a second Philox: 234 against 216 us for
+ * 16384 x 8192 bf16 with an fp32 residual.) N operands (0: nsrc of them, one by
+ * one) and the residual are all in flight before the numbers are computed. A
+ * block is one wave: 206 us there against 216 with four.
  *
  * `inv` is 2^64 / cols rounded up (unused for one column): the quotient by
  * cols is its high product, or one less (the rounding adds i * e / 2^64 < 1
@@ -328,22 +329,20 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
         return;
     }
     const int64_t i = begin + (int64_t)lane * V;         /* of the lane's first tile */
-    const bool whole = i >= 0 && i + (TL - 1) * 64 * V + V <= (int64_t)n;
-
+    bool whole[TL];                   /* whether a tile's vector lies in the call */
     T x[NN][TL][V];
     R r[TL][V];
-    if (whole) {
 #pragma unroll
-        for (int m = 0; m < NN; m++) {
+    for (int j = 0; j < TL; j++) {
+        const int64_t at = i + j * 64 * V;
+        whole[j] = at >= 0 && at + V <= (int64_t)n;
+        if (whole[j]) {
 #pragma unroll
-            for (int j = 0; j < TL; j++) {
-                load_raw<T, V>(static_cast<const T*>(srcs.p[m]) + i + j * 64 * V, x[m][j]);
+            for (int m = 0; m < NN; m++) {
+                load_raw<T, V>(static_cast<const T*>(srcs.p[m]) + at, x[m][j]);
             }
-        }
-        if (residual != nullptr) {
-#pragma unroll
-            for (int j = 0; j < TL; j++) {
-                load_raw<R, V>(residual + i + j * 64 * V, r[j]);
+            if (residual != nullptr) {
+                load_raw<R, V>(residual + at, r[j]);
             }
         }
     }
@@ -375,7 +374,7 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
             col = a - __umul64hi(a, inv) * cols;
             col = cols == 1 ? 0 : (int64_t)col < 0 ? col + cols : col;
         }
-        if (whole) {
+        if (whole[j]) {
             float s[V];
 #pragma unroll
             for (int k = 0; k < V; k++) {
@@ -400,7 +399,7 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
             if (bias != nullptr) {
                 if (col + V <= cols) {
                     T b[V];
-                    __builtin_memcpy(b, bias + col, sizeof(b));  /* temporal: every row's */
+                    load_raw<T, V, false>(bias + col, b);  /* temporal: every row's */
 #pragma unroll
                     for (int k = 0; k < V; k++) {
                         s[k] += (float)b[k];
@@ -767,10 +766,19 @@ k_balance(const T *logits, const I *index, const uint8_t *mask, Balance p, Balan
             if ((int64_t)named[u] >= 0 && (int64_t)named[u] < (int64_t)E) {
                 atomicAdd(&hist[named[u]], 1u);
             }
-            for (unsigned k = l + G; k < p.topk; k += G) {
-                const int64_t e = (int64_t)index[q * p.ld_index + k];
-                if (e >= 0 && e < (int64_t)E) {
-                    atomicAdd(&hist[e], 1u);
+            for (unsigned k0 = l + G; k0 < p.topk; k0 += 4 * G) {
+                I more[4];
+#pragma unroll
+                for (unsigned i = 0; i < 4; i++) {
+                    const unsigned k = k0 + i * G;
+                    more[i] = index[q * p.ld_index + (k < p.topk ? k : k0)];
+                }
+#pragma unroll
+                for (unsigned i = 0; i < 4; i++) {
+                    const int64_t e = (int64_t)more[i];
+                    if (k0 + i * G < p.topk && e >= 0 && e < (int64_t)E) {
+                        atomicAdd(&hist[e], 1u);
+                    }
                 }
             }
             float x[C], inv, lse;
@@ -1027,9 +1035,9 @@ __device__ __forceinline__ float exp_of(float x)
     return __builtin_amdgcn_exp2f(x * kLog2e);
 }
 
-/* exp(q) - q - 1, by its series near nought, where the subtractions would
- * leave nothing (to q^10 / 10!: the rest is below 5e-9 of it there) */
-__device__ __forceinline__ float exp_less(float q)
+/* (exp(q) - q - 1) / q^2 by its series, for |q| < 0.75, where the subtractions
+ * would leave nothing (to q^8 / 10!: the rest is below 5e-9 of it there) */
+__device__ __forceinline__ float exp_series(float q)
 {
     float s = 1.f / 3628800.f;
     s = __builtin_fmaf(s, q, 1.f / 362880.f);
@@ -1039,9 +1047,23 @@ __device__ __forceinline__ float exp_less(float q)
     s = __builtin_fmaf(s, q, 1.f / 120.f);
     s = __builtin_fmaf(s, q, 1.f / 24.f);
     s = __builtin_fmaf(s, q, 1.f / 6.f);
-    s = __builtin_fmaf(s, q, 0.5f) * q * q;
-    float e = exp_of(q) - q - 1.f;
-    asm("" : "+v"(s), "+v"(e));       /* both computed: no branch around either */
+    return __builtin_fmaf(s, q, 0.5f);
+}
+
+/* exp(q) - q - 1; both forms are computed: no branch around either */
+__device__ __forceinline__ float exp_less(float q)
+{
+    float s = exp_series(q) * q * q, e = exp_of(q) - q - 1.f;
+    asm("" : "+v"(s), "+v"(e));
+    return fabsf(q) < 0.75f ? s : e;
+}
+
+/* exp(q) - 1, to the end of its range (a reference of -inf or of the type's
+ * lowest value gives -1) */
+__device__ __forceinline__ float exp_minus(float q)
+{
+    float s = __builtin_fmaf(exp_series(q) * q, q, q), e = exp_of(q) - 1.f;
+    asm("" : "+v"(s), "+v"(e));
     return fabsf(q) < 0.75f ? s : e;
 }
 
@@ -1282,8 +1304,8 @@ constexpr int kSingleParts = 1024;
 
 template <typename T, bool REF, bool ROW, bool LINES, int NT>
 __global__ void __launch_bounds__(NT)
-k_policy(PolicyIn<T, REF, ROW, LINES> in, Policy p, PolicyPart *part, unsigned *done, float *sums, int64_t *counts,
-         int32_t *row_tokens, float *loss)
+k_policy(PolicyIn<T, REF, ROW, LINES> in, Policy p, PolicyPart *part, unsigned *done,
+         float *sums, int64_t *counts, int32_t *row_tokens, float *loss)
 {
     constexpr int V = 16 / sizeof(T), S = policy_steps<T>(), W = NT / 64;
     constexpr bool single = NT == kSingle;
@@ -1384,7 +1406,7 @@ __device__ __forceinline__ void policy_slope(const Tokens<T, V> &t, const Advant
         float g = (a.cuts(d) ? 0.f : r) * -a.a;
         if constexpr (REF) {
             const float q = (float)t.ref[k] - x;
-            g = __builtin_fmaf(-p.kl_coef, exp_less(q) + q, g);       /* 1 - exp(q) */
+            g = __builtin_fmaf(-p.kl_coef, exp_minus(q), g);
         }
         asm("" : "+v"(g));
         o[k] = t.live[k] != 0 ? g * w : 0.f;
