@@ -68,9 +68,15 @@ BalanceParams = struct.Struct("@iiNNNNNNdd").pack      # ucg_builtin_dev_balance
 PolicyParams = struct.Struct("@iiiNNNddd").pack        # ucg_builtin_dev_policy_params_t
 
 
+_POINTERS = [struct.Struct(f"@{n}P").pack for n in range(17)]
+
+
 def addresses(ptrs):
     """a C array of pointers (None: NULL)"""
-    return struct.pack(f"{len(ptrs)}P", *(p or 0 for p in ptrs))
+    try:
+        return _POINTERS[len(ptrs)](*ptrs)
+    except (struct.error, IndexError):
+        return struct.pack(f"@{len(ptrs)}P", *(p or 0 for p in ptrs))
 
 
 ZCOPY_NEVER = (1 << 64) - 1   # UCG_BUILTIN_DEV_ZCOPY_NEVER

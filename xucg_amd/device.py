@@ -256,11 +256,13 @@ class DevContext:
         if x is None or x.__class__ is int:
             return x
         try:
-            dtype = x.dtype
-            address = x.data_ptr()
+            dtype, address = x.dtype, x.data_ptr()
         except AttributeError:
             return _ptr(x)
-        if dtype is not _TORCH.get(dt) and not _is_dtype(dtype, dt):
+        if (step == row and x.is_contiguous() and x.numel() == n and
+                dtype is _TORCH.get(dt) and x.get_device() == self.device):
+            return address
+        if not _is_dtype(dtype, dt):
             raise ValueError(f"{name}: {dt} wanted, got {dtype}")
         if x.get_device() != self.device:
             raise ValueError(f"{name}: a tensor on cuda:{self.device} wanted, got {x.device}")
