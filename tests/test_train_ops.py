@@ -149,7 +149,8 @@ def test_sum_dropout_refusals():
     bad("overlaps a source", P(), dst=PTR + 4)
     bad("overlaps a source", P("bfloat16", "float32"), dst=PTR)
     bad("overlaps the residual", P(), res=2 * PTR + 4)
-    bad("overlaps the residual or the bias", P(), bias=2 * PTR + 64)
+    bad("overlaps the residual, the bias or rng", P(), bias=2 * PTR + 64)
+    bad("overlaps the residual, the bias or rng", P(rng=2 * PTR + 64))
     # what is allowed comes as far as the missing context
     bad("ctx is NULL", P(), dst=PTR)
     bad("ctx is NULL", P(), res=2 * PTR)
@@ -217,10 +218,17 @@ def test_balance_refusals():
     bad("misaligned", P(), counts=3 * M + 4)
     bad("workspace", P(tokens=1 << 20))
     bad("workspace", P(tokens=1 << 20), ws=5 * M, n=need - 1)
+    bad("overlapping", P(), counts=M)
+    bad("overlapping", P(), sums=2 * M)
+    bad("overlapping", P(), sums=3 * M + 64)
+    bad("overlapping", P(), loss=4 * M)
+    bad("overlapping", P(), mask=3 * M)
+    bad("overlapping", P(tokens=1 << 20), ws=4 * M, n=need)
     bad("ctx is NULL", P(tokens=1 << 20), ws=5 * M, n=need)
     bad("ctx is NULL", P(tokens=0), logits=None, index=None)
     refused("ucg_builtin_dev_balance_loss", INVALID, "NULL", P(), None, M, M)
-    refused("ucg_builtin_dev_balance_loss", INVALID, "ctx is NULL", P(), M, M, M)
+    refused("ucg_builtin_dev_balance_loss", INVALID, "overlapping", P(), M, 2 * M, M)
+    refused("ucg_builtin_dev_balance_loss", INVALID, "ctx is NULL", P(), M, 2 * M, 3 * M)
 
     def badg(why, q, logits=M, mask=None, counts=3 * M, base=None, g=None, d=5 * M, status=INVALID):
         refused("ucg_builtin_dev_balance_grad", status, why, q, logits, mask, counts, base, g, d)
@@ -260,8 +268,13 @@ def test_policy_refusals():
     bad("misaligned", P(), counts=5 * M + 4)
     bad("workspace", P(), ws=None)
     bad("workspace", P(), n=need - 1)
+    bad("overlapping", P(), sums=M)
+    bad("overlapping", P(), rt=5 * M + 16)
+    bad("overlapping", P(per_row=1), ws=3 * M)
+    bad("overlapping", P(), loss=4 * M)
     bad("ctx is NULL", P())
     refused("ucg_builtin_dev_policy_loss", INVALID, "NULL", P(), M, M, None)
+    refused("ucg_builtin_dev_policy_loss", INVALID, "overlapping", P(), M, 2 * M, M)
 
     def badg(why, q, logp=M, old=2 * M, ref=None, adv=3 * M, mask=None, rt=None, counts=5 * M,
              g=None, d=7 * M, status=INVALID):
@@ -276,6 +289,34 @@ def test_policy_refusals():
     badg("overlaps", P(), mask=7 * M)
     badg("ctx is NULL", P(), d=M)
     badg("ctx is NULL", P(), d=2 * M)
+
+
+def test_python_refusals():
+    """What is no device memory, too small a buffer, numbers that no size is."""
+    ctx = xucg_amd.DevContext.__new__(xucg_amd.DevContext)   # no GPU is needed to refuse
+    ctx.handle, ctx.device = None, 0
+    buf = xucg_amd.DevBuffer.__new__(xucg_amd.DevBuffer)
+    buf.ptr, buf.nbytes = PTR, 4 * 32
+    x = np.zeros(32, np.float32)
+    with pytest.raises(TypeError, match="dst"):
+        ctx.sum_dropout("float32", x, [PTR], 4, 8, 0.1, 1)
+    with pytest.raises(TypeError, match="srcs"):
+        ctx.sum_dropout("float32", PTR, [x], 4, 8, 0.1, 1)
+    with pytest.raises(ValueError, match="dst"):
+        ctx.sum_dropout("float32", buf, [2 * PTR], 4, 9, 0.1, 1)
+    with pytest.raises(ValueError, match="logits"):
+        ctx.balance("float32", buf, PTR, 4, 8, 2, PTR, PTR, ld=9)
+    for bad in (dict(rows=-1), dict(p="x"), dict(seed=-1), dict(rows=1.5)):
+        kw = dict(dict(rows=4, p=0.1, seed=1), **bad)
+        with pytest.raises((ValueError, TypeError)):
+            ctx.sum_dropout("float32", PTR, [2 * PTR], kw["rows"], 8, kw["p"], kw["seed"])
+    with pytest.raises(xucg_amd.UcsError, match="NULL or misaligned source"):
+        ctx.sum_dropout("float32", PTR, [None], 4, 8, 0.1, 1)
+    with pytest.raises(xucg_amd.UcsError, match="nsrc must be"):
+        ctx.sum_dropout("float32", PTR, [2 * PTR] * 17, 4, 8, 0.1, 1)
+    with pytest.raises(KeyError):
+        ctx.sum_dropout("float31", PTR, [2 * PTR], 4, 8, 0.1, 1)
+    buf.ptr = None                       # nothing to free
 
 
 def test_row_bounds_cover():

@@ -63,9 +63,22 @@ BALANCE_FIELDS = ("dt", "index_dt", "tokens", "experts", "topk", "ld", "ld_index
                   "balance_coef", "z_coef")
 POLICY_FIELDS = ("dt", "adv_per_row", "per_sequence", "rows", "cols", "ld", "clip_low",
                  "clip_high", "kl_coef")
-DropoutParams = struct.Struct("@iiNNdQQQP").pack       # ucg_builtin_dev_dropout_params_t
-BalanceParams = struct.Struct("@iiNNNNNNdd").pack      # ucg_builtin_dev_balance_params_t
-PolicyParams = struct.Struct("@iiiNNNddd").pack        # ucg_builtin_dev_policy_params_t
+
+
+def _packer(layout, fields):
+    pack = struct.Struct(layout).pack
+
+    def params(*values):
+        try:
+            return pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f"{', '.join(fields)} = {values}: {e}") from None
+    return params
+
+
+DropoutParams = _packer("@iiNNdQQQP", DROPOUT_FIELDS)    # ucg_builtin_dev_dropout_params_t
+BalanceParams = _packer("@iiNNNNNNdd", BALANCE_FIELDS)   # ucg_builtin_dev_balance_params_t
+PolicyParams = _packer("@iiiNNNddd", POLICY_FIELDS)      # ucg_builtin_dev_policy_params_t
 
 
 _POINTERS = [struct.Struct(f"@{n}P").pack for n in range(17)]

@@ -10,6 +10,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 #include "ucg_builtin_dev.h"
 #include "dev_internal.h"
 #include "dev_kernels.h"
@@ -1545,6 +1547,33 @@ bool overlap(const void *a, size_t na, const void *b, size_t nb)
     return na != 0 && nb != 0 && x < y + nb && y < x + na;
 }
 
+struct Range {
+    const void *p;
+    size_t      bytes;
+};
+
+/* whether an output shares bytes with another output or with an input (NULL
+ * ranges share none) */
+bool clash(std::initializer_list<Range> outs, std::initializer_list<Range> ins)
+{
+    for (const Range *a = outs.begin(); a != outs.end(); a++) {
+        if (a->p == nullptr) {
+            continue;
+        }
+        for (const Range *b = a + 1; b != outs.end(); b++) {
+            if (b->p != nullptr && overlap(a->p, a->bytes, b->p, b->bytes)) {
+                return true;
+            }
+        }
+        for (const Range &b : ins) {
+            if (b.p != nullptr && overlap(a->p, a->bytes, b.p, b.bytes)) {
+                return true;
+            }
+        }
+    }
+    return false;
+}
+
 /* rows x cols elements of `size` bytes, a row every ld: their span in bytes.
  * False when that does not fit in 63 bits. */
 bool span(uint64_t rows, uint64_t cols, uint64_t ld, size_t size, size_t *bytes)
@@ -1924,9 +1953,9 @@ ucs_status_t ucg_builtin_dev_sum_dropout(ucg_builtin_dev_ctx_t *ctx,
                 return invalid(what, "dst overlaps a source");
             }
         }
-        if ((residual != dst && residual != nullptr && overlap(dst, n * rs, residual, n * rs)) ||
-            (bias != nullptr && overlap(dst, n * rs, bias, params->cols * ts))) {
-            return invalid(what, "dst overlaps the residual or the bias");
+        if (clash({{dst, n * rs}}, {{residual != dst ? residual : nullptr, n * rs},
+                                    {bias, params->cols * ts}, {params->rng, 16}})) {
+            return invalid(what, "dst overlaps the residual, the bias or rng");
         }
     }
     if (ctx == nullptr) {
@@ -1987,11 +2016,9 @@ ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
         return invalid(what, "the workspace is missing or too small");
     }
     if (((dsrc != grad || ts != rs) && overlap(dsrc, n * ts, grad, n * rs)) ||
-        (dbias != nullptr &&
-         (overlap(dbias, cols * 4, dsrc, n * ts) || overlap(dbias, cols * 4, grad, n * rs))) ||
-        (need != 0 && (overlap(workspace, need, dsrc, n * ts) ||
-                       overlap(workspace, need, grad, n * rs) ||
-                       overlap(workspace, need, dbias, cols * 4)))) {
+        clash({{dsrc, n * ts}, {dbias, cols * 4}, {need ? workspace : nullptr, need}},
+              {{params->rng, 16}}) ||
+        clash({{dbias, cols * 4}, {need ? workspace : nullptr, need}}, {{grad, n * rs}})) {
         return invalid(what, "overlapping buffers");
     }
     if (ctx == nullptr) {
@@ -2076,6 +2103,11 @@ ucs_status_t ucg_builtin_dev_balance(ucg_builtin_dev_ctx_t *ctx,
     if (need != 0 && (workspace == nullptr || workspace_bytes < need)) {
         return invalid(what, "the workspace is missing or too small");
     }
+    if (clash({{counts, (b.experts + 1) * sizeof(int64_t)}, {sums, (b.experts + 1) * sizeof(float)},
+               {loss, 3 * sizeof(float)}, {need ? workspace : nullptr, need}},
+              {{logits, bytes}, {index, index_bytes}, {mask, b.tokens}})) {
+        return invalid(what, "overlapping buffers");
+    }
     if (ctx == nullptr) {
         return invalid(what, "ctx is NULL");
     }
@@ -2135,6 +2167,10 @@ ucs_status_t ucg_builtin_dev_balance_loss(ucg_builtin_dev_ctx_t *ctx,
         misaligned(sums, 4) || misaligned(loss, 4)) {
         return invalid(what, "NULL or misaligned buffer");
     }
+    if (clash({{loss, 3 * sizeof(float)}}, {{counts, (b.experts + 1) * sizeof(int64_t)},
+                                            {sums, (b.experts + 1) * sizeof(float)}})) {
+        return invalid(what, "overlapping buffers");
+    }
     if (ctx == nullptr) {
         return invalid(what, "ctx is NULL");
     }
@@ -2173,10 +2209,10 @@ ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
         return invalid(what, "misaligned buffer");
     }
     if (((dlogits != logits || b.ld != b.ld_out) && overlap(dlogits, out_bytes, logits, bytes)) ||
-        (base != nullptr && dlogits != base && overlap(dlogits, out_bytes, base, out_bytes)) ||
-        (mask != nullptr && overlap(dlogits, out_bytes, mask, b.tokens)) ||
-        overlap(dlogits, out_bytes, counts, (b.experts + 1) * 8) ||
-        (grad_loss != nullptr && overlap(dlogits, out_bytes, grad_loss, 4))) {
+        clash({{dlogits, out_bytes}}, {{base != dlogits ? base : nullptr, out_bytes},
+                                       {mask, b.tokens},
+                                       {counts, (b.experts + 1) * sizeof(int64_t)},
+                                       {grad_loss, sizeof(float)}})) {
         return invalid(what, "dlogits overlaps an input");
     }
     if (ctx == nullptr) {
@@ -2247,6 +2283,13 @@ ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
     if (workspace == nullptr || workspace_bytes < need) {
         return invalid(what, "the workspace is missing or too small");
     }
+    const size_t nb = bytes / 4 * ts;
+    if (clash({{sums, 2 * sizeof(float)}, {counts, 3 * sizeof(int64_t)}, {row_tokens, p.rows * 4},
+               {loss, 3 * sizeof(float)}, {workspace, need}},
+              {{logp, nb}, {old, nb}, {ref, nb}, {mask, bytes / 4},
+               {adv, params->adv_per_row ? p.rows * 4 : bytes}})) {
+        return invalid(what, "overlapping buffers");
+    }
     if (ctx == nullptr) {
         return invalid(what, "ctx is NULL");
     }
@@ -2312,6 +2355,10 @@ ucs_status_t ucg_builtin_dev_policy_loss(ucg_builtin_dev_ctx_t *ctx,
         misaligned(sums, 4) || misaligned(loss, 4)) {
         return invalid(what, "NULL or misaligned buffer");
     }
+    if (clash({{loss, 3 * sizeof(float)}}, {{counts, 3 * sizeof(int64_t)},
+                                            {sums, 2 * sizeof(float)}})) {
+        return invalid(what, "overlapping buffers");
+    }
     if (ctx == nullptr) {
         return invalid(what, "ctx is NULL");
     }
@@ -2350,14 +2397,11 @@ ucs_status_t ucg_builtin_dev_policy_grad(ucg_builtin_dev_ctx_t *ctx,
         misaligned(row_tokens, 4) || misaligned(grad_loss, 4)) {
         return invalid(what, "misaligned buffer");
     }
-    if ((dlogp != logp && overlap(dlogp, nb, logp, nb)) ||
-        (dlogp != old && overlap(dlogp, nb, old, nb)) ||
-        (ref != nullptr && dlogp != ref && overlap(dlogp, nb, ref, nb)) ||
-        overlap(dlogp, nb, adv, params->adv_per_row ? p.rows * 4 : bytes) ||
-        (mask != nullptr && overlap(dlogp, nb, mask, bytes / 4)) ||
-        (row_tokens != nullptr && overlap(dlogp, nb, row_tokens, p.rows * 4)) ||
-        (grad_loss != nullptr && overlap(dlogp, nb, grad_loss, 4)) ||
-        overlap(dlogp, nb, counts, 24)) {
+    if (clash({{dlogp, nb}}, {{logp != dlogp ? logp : nullptr, nb}, {old != dlogp ? old : nullptr, nb},
+                              {ref != dlogp ? ref : nullptr, nb}, {mask, bytes / 4},
+                              {adv, params->adv_per_row ? p.rows * 4 : bytes},
+                              {row_tokens, p.rows * 4}, {counts, 3 * sizeof(int64_t)},
+                              {grad_loss, sizeof(float)}})) {
         return invalid(what, "dlogp overlaps an input");
     }
     if (ctx == nullptr) {

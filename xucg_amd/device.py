@@ -258,7 +258,12 @@ class DevContext:
         try:
             dtype, address = x.dtype, x.data_ptr()
         except AttributeError:
-            return _ptr(x)
+            if not isinstance(x, (DevBuffer, HostBuffer)):
+                raise TypeError(f"{name}: device memory wanted, got {type(x)}") from None
+            span = n if step == row or not n else (n // row - 1) * step + row
+            if span * DTYPE_SIZE[_DT[dt]] > x.nbytes:
+                raise ValueError(f"{name}: a buffer of {span} {dt} wanted, got {x.nbytes} bytes")
+            return x.ptr
         if (step == row and x.is_contiguous() and x.numel() == n and
                 dtype is _TORCH.get(dt) and x.get_device() == self.device):
             return address
