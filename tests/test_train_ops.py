@@ -291,6 +291,30 @@ def test_policy_refusals():
     badg("ctx is NULL", P(), d=2 * M)
 
 
+def test_kernels_keep_off_scratch_and_packed_fp32():
+    """No kernel of dev_train.hip spills or indexes into scratch memory, and none
+    holds a packed fp32 instruction (read from the built object)."""
+    import re
+    llvm, obj = "/opt/rocm/lib/llvm/bin", os.path.join(ROOT, "xucg_amd", "csrc", "_obj", "dev_train.o")
+    if not os.path.exists(obj) or not os.path.exists(f"{llvm}/clang-offload-bundler"):
+        pytest.skip("the device object is not built here")
+    import tempfile
+    with tempfile.TemporaryDirectory() as d:
+        fb, co = os.path.join(d, "fb"), os.path.join(d, "co")
+        subprocess.run([f"{llvm}/llvm-objcopy", f"--dump-section=.hip_fatbin={fb}", obj,
+                        os.path.join(d, "junk")], check=True, capture_output=True)
+        subprocess.run([f"{llvm}/clang-offload-bundler", "--type=o", "--unbundle",
+                        "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--input={fb}", f"--output={co}"],
+                       check=True, capture_output=True)
+        notes = subprocess.run([f"{llvm}/llvm-readelf", "--notes", co], check=True, capture_output=True,
+                               text=True).stdout
+        code = subprocess.run([f"{llvm}/llvm-objdump", "-d", "--no-show-raw-insn", co], check=True,
+                              capture_output=True, text=True).stdout
+    scratch = [int(x) for x in re.findall(r"\.private_segment_fixed_size:\s+(\d+)", notes)]
+    assert len(scratch) > 100 and not any(scratch)
+    assert not re.search(r"v_pk_(add|mul|fma)_f32", code) and "v_bitop3_b32" in code
+
+
 def test_python_refusals():
     """What is no device memory, too small a buffer, numbers that no size is."""
     ctx = xucg_amd.DevContext.__new__(xucg_amd.DevContext)   # no GPU is needed to refuse
