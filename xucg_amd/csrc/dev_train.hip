@@ -541,21 +541,35 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
                 }
             }
         }
-    } else if (c < cols) {            /* not SPLIT: there a vector is in or out */
+    } else if (!SPLIT && c < cols) {  /* the row's last columns, fewer than eight: a lane,
+                                       * which has the next row's on the way */
+        const R *from = grad + ((uint64_t)blockIdx.y * ty + y) * cols;
+        R g[8];
+        if ((uint64_t)blockIdx.y * ty + y < rows) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                g[k] = from[c + k < cols ? c + k : cols - 1];
+            }
+        }
         for (uint64_t q = (uint64_t)blockIdx.y * ty + y; q < rows; q += step) {
+            R next[8];
+            from = grad + (q + step < rows ? q + step : q) * cols;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                next[k] = from[c + k < cols ? c + k : cols - 1];
+            }
             uint32_t u[4] = {};
             if (rng.threshold != 0) {
                 draw<ALIGNED>(rng.offset + q * cols + c, tag, seed, u);
             }
+            float d[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                if (c + k < cols) {
-                    const float d = kept(u, k, rng.threshold)
-                                        ? (float)grad[q * cols + c + k] * rng.scale : 0.f;
-                    sum[k] += d;
-                    dsrc[q * cols + c + k] = (T)d;
-                }
+                d[k] = kept(u, k, rng.threshold) ? (float)g[k] * rng.scale : 0.f;
+                sum[k] += d[k];           /* what is past the row is not written */
             }
+            store_row<T, 8>(dsrc + q * cols, c, cols, d);
+            __builtin_memcpy(g, next, sizeof(g));
         }
     }
 #pragma unroll
@@ -1797,9 +1811,9 @@ ucs_status_t balance_check(const ucg_builtin_dev_balance_params_t *p, const char
 
 /* Blocks of k_balance: one to a CU at most, and to be joined at once. One block
  * does up to 32768 logits by itself, which takes less than a second launch (200
- * tokens of 8 experts 4.5 against 8.5 us, 300 of 64 6.2 against 10.2, 4000 of 8 the
- * same); beyond, 128 rows a block at least (more rows in fewer blocks took
- * longer: 4096 of 64 12.1 against 10.3 us at 512 rows). */
+ * tokens of 8 experts 4.5 against 8.5 us, 300 of 64 6.2 against 7.7); beyond, a
+ * block has 2048 logits at least, in 16 to 128 rows (1000 tokens of 256 experts
+ * 8.6 us at 16 rows, 11.4 at 128; 3000 of 16 7.8 at 16 rows, 7.5 at 128). */
 void balance_plan(uint64_t tokens, uint64_t experts, uint64_t *blocks, uint64_t *chunk)
 {
     constexpr uint64_t kAlone = 32768;
@@ -1808,8 +1822,9 @@ void balance_plan(uint64_t tokens, uint64_t experts, uint64_t *blocks, uint64_t 
         *blocks = 1;
         return;
     }
-    const uint64_t c = div_up(tokens, kMaxParts);
-    *chunk  = c < 128 ? 128 : c;
+    const uint64_t c = div_up(tokens, kMaxParts), few = 2048 / experts;
+    const uint64_t least = few < 16 ? 16 : few > 128 ? 128 : few;
+    *chunk  = c < least ? least : c;
     *blocks = div_up(tokens, *chunk);
 }
 
