@@ -311,7 +311,7 @@ constexpr int kWaveElems = 512;
  * one) and the residual are all in flight before the numbers are computed. A
  * block is one wave: 206 us there against 216 with four.
  *
- * HBM bounds it: 16384 x 8192 bf16 with an fp32 residual takes 205 us = 6.5 TB/s
+ * HBM bounds it: 16384 x 8192 bf16 with an fp32 residual takes 206 us = 6.5 TB/s
  * (this library's plain copy reaches 6.8), four bf16 sources of 4096 x 4096 33.4
  * us = 6.0 TB/s; without the numbers (p = 0) it takes as long. Waves whose parts
  * begin inside a line share it with their neighbours: `map` deals them to the
@@ -468,7 +468,7 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
  * eight (ALIGNED 0: the columns or the offset are no multiple of eight): then
  * the eight are neighbours whose numbers come from two groups.
  *
- * 8192 x 4096 bf16 takes 24.4 us = 5.5 TB/s, and 4.9 for the join of 128 parts
+ * 8192 x 4096 bf16 takes 25.2 us = 5.3 TB/s, and 4.7 for the join of 128 parts
  * (less than half of a launch is its bytes); fp32 54 us with it = 5.0 TB/s. With
  * rows in chunks of neighbours instead of dealt to the parts fp32 took 63, with
  * the eight fp32 columns side by side 74 us. 8191 x 4097 bf16 takes 41 us: twice
@@ -741,7 +741,7 @@ constexpr int kBalanceThreads = 1024;  /* 16 waves: one block to a CU */
  * others (the mask is not waited for) and left out afterwards. Counts are
  * integers, so their LDS atomics give the same in any order.
  *
- * 65536 x 256 bf16, top 8: 11.2 us, and 5.3 with the loss for the join. Without the
+ * 65536 x 256 bf16, top 8: 11.7 us, and 4.7 with the loss for the join. Without the
  * softmax 8.6: the exponentials and sums of 16 M probabilities do not hide behind
  * 38 MB here, and 256 blocks start and end together. 512 of them take longer for
  * the join than they save (18.1 against 17.3 us in all). */
