@@ -789,6 +789,21 @@ def test_policy(dev_ctx, dt, rows, cols):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [5, 3000])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_policy_rows_without_columns_read_nothing(dev_ctx, rows, per_row):
+    s, c = Arr(dev_ctx, np.ones(2, np.float32)), Arr(dev_ctx, np.ones(3, np.int64))
+    rt, loss = Arr(dev_ctx, np.full(rows, -1, np.int32)), Arr(dev_ctx, np.ones(3, np.float32))
+    ws = dev_ctx.alloc(dev_ctx.policy_workspace(rows, 0))
+    dev_ctx.policy("bfloat16", None, None, None, rows, 0, s.ptr, c.ptr, row_tokens=rt.ptr,
+                   adv_per_row=per_row, per_sequence=True, loss=loss.ptr, workspace=ws)
+    dev_ctx.policy_grad("bfloat16", None, None, None, None, rows, 0, c.ptr, row_tokens=rt.ptr,
+                        adv_per_row=per_row, per_sequence=True)
+    dev_ctx.sync()
+    assert not s.get().any() and not c.get().any() and not rt.get().any() and not loss.get().any()
+
+
+@gpu
 def test_policy_clip_goes_by_the_difference(dev_ctx):
     """At a limit a token is not cut, one step beyond it is; A = 0 never is.
     clip_low = 1 never cuts below."""

@@ -2330,7 +2330,9 @@ ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
     /* one block does a few parts by itself: a second launch costs more */
     const bool single = grid.x * grid.y <= 4 && p.rows * p.chunks <= (uint64_t)kSingleParts;
     const bool lines = on_lines(p, ts, logp, old, ref);
-    with_policy(params->dt, ref != nullptr, params->adv_per_row != 0, lines && !single,
+    /* rows without columns: adv may be NULL, and is not read by rows either */
+    const bool by_row = params->adv_per_row != 0 && bytes != 0;
+    with_policy(params->dt, ref != nullptr, by_row, lines && !single,
                 [&](auto t, auto rf, auto rw, auto ln) {
         typedef decltype(t) T;
         constexpr bool REF = decltype(rf)::value, ROW = decltype(rw)::value;
