@@ -33,6 +33,7 @@
 #include <execinfo.h>
 #include <signal.h>
 #include <sys/socket.h>
+#include <sys/stat.h>
 #include <sys/un.h>
 #include <fcntl.h>
 #include <pthread.h>
@@ -586,6 +587,25 @@ hipError_t import_fd(hipMemGenericAllocationHandle_t *h, int fd, int device)
     return hipMemImportFromShareableHandle(h, (void*)(intptr_t)fd, t);
 }
 
+/* What tells the causes of a failed import apart, which the runtime reports
+ * with one status: whether the descriptor that arrived is open, and how large
+ * the object behind it is (a dma-buf answers SEEK_END with its size); and which
+ * convention this process found, on an import of its own that succeeded. */
+std::string import_failure(int fd)
+{
+    static const char *const conv[] = {"unknown", "value", "address"};
+    struct stat sb;
+    std::string s = "ipc_import: import of the peer's descriptor (";
+    if (fstat(fd, &sb) != 0) {
+        s += std::string("not open here: ") + strerror(errno);
+    } else {
+        const off_t n = lseek(fd, 0, SEEK_END);
+        s += n < 0 ? "open, of no known size" : "open, " + std::to_string((long long)n) + " bytes";
+    }
+    return s + "; descriptors are taken by " +
+           conv[g_fd_convention.load(std::memory_order_relaxed) + 1] + ")";
+}
+
 /* map an imported VMM allocation (fd) at a new reservation of this process */
 ucs_status_t va_room(size_t bytes, const char *what);
 void va_unclaim(size_t bytes);
@@ -600,7 +620,7 @@ ucs_status_t map_vmm(int fd, size_t size, int device, import_rec *m)
     hipError_t e = import_fd(&h, fd, device);
     if (e != hipSuccess) {
         va_unclaim(size);
-        return hip_status(e, "import_fd(&h, fd, device)");
+        return hip_status(e, import_failure(fd).c_str());
     }
     void *va = nullptr;
     e = hipMemAddressReserve(&va, size, kGran, nullptr, 0);
