@@ -2327,8 +2327,10 @@ ucs_status_t ucg_builtin_dev_policy(ucg_builtin_dev_ctx_t *ctx,
     HIP_TRY(dev.err);
     hipStream_t stream = stream_of(ctx);
     const dim3 grid    = policy_grid(p, kThreads / 64);
-    /* one block does a few parts by itself: a second launch costs more */
-    const bool single = grid.x * grid.y <= 4 && p.rows * p.chunks <= (uint64_t)kSingleParts;
+    /* one block does a few parts by itself: a second launch costs more. Without
+     * rows it has none, however many a row would have, and writes the zeros. */
+    const bool single = p.rows == 0 || (grid.x * grid.y <= 4 &&
+                                        p.rows * p.chunks <= (uint64_t)kSingleParts);
     const bool lines = on_lines(p, ts, logp, old, ref);
     /* rows without columns: adv may be NULL, and is not read by rows either */
     const bool by_row = params->adv_per_row != 0 && bytes != 0;
