@@ -8,7 +8,7 @@ import pytest
 
 import xucg_amd
 from oracle import train_ref as R
-from test_train_ops import DTS, U, Arr, gpu, ptr
+from test_train_ops import DTS, U, Arr, balance_bounds, gpu, ptr
 from xucg_amd import group as G
 
 
@@ -42,3 +42,34 @@ def test_policy_of_a_member_without_rows(dev_ctx, dt, cols):
     dev_ctx.sync()
     assert sorted(joined) == ["float32", "int64"]
     assert c.get().tolist() == [4, 2, 1] and loss.get().tolist() == [1.875, 1.5, 0.75]
+
+
+# ---- the balance gradient's centre ---------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("experts,topk,dropped", [(64, 8, 0.5), (60, 8, 0.9), (512, 4, 0.3), (1000, 2, 0.97)])
+def test_balance_grad_of_dropped_choices(dev_ctx, dt, experts, topk, dropped):
+    """Counts that are near one another and far below tokens * topk / experts:
+    choices with an index outside the experts are counted nowhere. The
+    gradient's p (c - p.c) needs the counts' differences alone, so its bound
+    goes by their spread: each term of the dot has the spread, the error of a
+    probability and one rounding for itself and each of its sums."""
+    rng = np.random.default_rng(experts)
+    tokens, members = 40, 1 << 16
+    x = R.from_storage(R.to_storage(rng.normal(size=(tokens, experts)), dt), dt)
+    mean = int(members * topk * (1 - dropped) / experts)
+    counts = np.append(mean + rng.integers(-3, 4, experts), members).astype(np.int64)
+    la, ca, d = Arr(dev_ctx, R.to_storage(x, dt)), Arr(dev_ctx, counts), Arr(dev_ctx, R.to_storage(np.zeros_like(x), dt))
+    coef = float(members) ** 2 / experts        # the result is of the counts' own size
+    dev_ctx.balance_grad(dt, d.ptr, la.ptr, tokens, experts, topk, ca.ptr, balance_coef=coef)
+    dev_ctx.sync()
+    want = R.balance_grad(x, None, counts, topk, coef, 0.0)
+    rel, _ = balance_bounds(x, None)
+    p, _ = R.softmax(x)
+    # differences of two counts: 6 at most
+    size = 8 * coef * experts / topk / float(members) ** 2
+    tol = p * size * (2 * rel + (experts + 8) * U)
+    off = np.abs(R.from_storage(d.get(), dt) - want)
+    tol = tol + R.EPS[dt] * (np.abs(want) + tol) * 1.01 + R.LEAST[dt]
+    assert (off <= tol).all(), (off / tol).max()
+
