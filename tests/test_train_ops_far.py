@@ -73,3 +73,26 @@ def test_balance_grad_of_dropped_choices(dev_ctx, dt, experts, topk, dropped):
     tol = tol + R.EPS[dt] * (np.abs(want) + tol) * 1.01 + R.LEAST[dt]
     assert (off <= tol).all(), (off / tol).max()
 
+
+
+# ---- many rows to a lane -------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dt,rows,cols,offset", [
+    ("float32", 1 << 21, 8, 0), ("float32", 1 << 21, 8, 3), ("float32", 1 << 18, 65, 1),
+    ("bfloat16", 1 << 20, 16, 0), ("bfloat16", 300, (1 << 19) + 8, 0), ("bfloat16", 300, (1 << 19) + 3, 0)])
+def test_bias_gradient_of_many_rows(dev_ctx, dt, rows, cols, offset):
+    """Columns that begin with ones and go on with values that a sum of 1 in 32
+    bits loses whole. At most 32 rows are added up in 32 bits, a part and the
+    result are rounded once more: 33 u of the sum of sizes."""
+    head = min(rows // 64, 1 << 15)
+    one, small = R.to_storage(np.array([1.0, 2.0 ** -24]), dt)
+    g = np.full((rows, cols), small)
+    g[:head] = one
+    ga, d = Arr(dev_ctx, g), Arr(dev_ctx, np.zeros_like(g))
+    db = Arr(dev_ctx, np.ones(cols, np.float32))
+    ws = dev_ctx.alloc(max(16, dev_ctx.sum_dropout_grad_workspace(rows, cols)))
+    dev_ctx.sum_dropout_grad(dt, d.ptr, ga.ptr, rows, cols, 0.0, 1, offset=offset, dbias=db.ptr, workspace=ws)
+    dev_ctx.sync()
+    want = head + (rows - head) * 2.0 ** -24
+    assert np.abs(db.get() - want).max() <= 33 * U * want
+    assert (d.get() == g).all()

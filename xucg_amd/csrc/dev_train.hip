@@ -468,20 +468,30 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
  * eight (ALIGNED 0: the columns or the offset are no multiple of eight): then
  * the eight are neighbours whose numbers come from two groups.
  *
+ * Sums: a lane's rows in 32 bits, at most kFewRows of them; with more (DEEP) the
+ * four of a pass, and passes in 64, for which it needs 12 registers more (8191 x
+ * 4097 bf16, 18 rows a lane, 40.9 us without and 41.7 with it; 2^20 x 64 bf16, 128
+ * rows, 68.0 and 69.0). Lanes of a column are joined in 64 bits, a part is
+ * rounded to 32 (half the join's bytes: 8192 x 4096 bf16 27.7 us, 28.1 in 64),
+ * parts are joined in 64.
+ *
  * 8192 x 4096 bf16 takes 25.2 us = 5.3 TB/s, and 4.7 for the join of 128 parts
  * (less than half of a launch is its bytes); fp32 54 us with it = 5.0 TB/s. With
  * rows in chunks of neighbours instead of dealt to the parts fp32 took 63, with
  * the eight fp32 columns side by side 74 us. 8191 x 4097 bf16 takes 41 us: twice
  * the Philox rounds, and a block column of one column.
  */
-template <typename R, typename T, bool ALIGNED>
+constexpr unsigned kFewRows = 32;
+
+template <typename R, typename T, bool ALIGNED, bool DEEP>
 __global__ void __launch_bounds__(kThreads)
 k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t cols,
                unsigned tx, Rng rng)
 {
     constexpr bool SPLIT = ALIGNED && (sizeof(R) == 4 || sizeof(T) == 4);
     constexpr int U = 4, TL = SPLIT ? 2 : 1, V = 8 / TL;
-    __shared__ float lds[kThreads * 8];
+    typedef typename std::conditional<DEEP, double, float>::type S;
+    __shared__ S lds[kThreads * 8];
     const unsigned x  = threadIdx.x % tx, y = threadIdx.x / tx, ty = kThreads / tx;
     const uint64_t c0 = (uint64_t)blockIdx.x * tx * 8;          /* the block's first column */
     const uint64_t c  = c0 + x * V, tile = (uint64_t)tx * V;
@@ -490,7 +500,7 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
     const uint64_t step = (uint64_t)gridDim.y * ty;
     uint64_t seed, tag;
     rng_state(rng, seed, tag);
-    float sum[8] = {};
+    S sum[8] = {};
     bool has[TL];                     /* whether a tile's vector lies in the row */
 #pragma unroll
     for (int j = 0; j < TL; j++) {
@@ -509,6 +519,11 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
                     load_raw<R, V>(grad + (q < rows ? q : row) * cols + c + (has[h] ? h * tile : 0),
                                    g[j][h]);
                 }
+            }
+            float few[8];             /* the sums that these rows go on with */
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                few[k] = DEEP ? 0.f : (float)sum[k];
             }
 #pragma unroll
             for (int j = 0; j < U; j++) {
@@ -532,13 +547,17 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
                         for (int k = 0; k < V; k++) {
                             d[k] = kept(u, h * V + k, rng.threshold)
                                        ? (float)g[j][h][k] * rng.scale : 0.f;
-                            sum[h * V + k] += d[k];
+                            few[h * V + k] += d[k];
                         }
                         if (has[h]) {
                             store_vec<T, V>(dsrc + q * cols + c + h * tile, d);
                         }
                     }
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                sum[k] = DEEP ? sum[k] + (S)few[k] : (S)few[k];
             }
         }
     } else if (!SPLIT && c < cols) {  /* the row's last columns, fewer than eight: a lane,
@@ -566,7 +585,7 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 d[k] = kept(u, k, rng.threshold) ? (float)g[k] * rng.scale : 0.f;
-                sum[k] += d[k];           /* what is past the row is not written */
+                sum[k] += (S)d[k];        /* what is past the row is not written */
             }
             store_row<T, 8>(dsrc + q * cols, c, cols, d);
             __builtin_memcpy(g, next, sizeof(g));
@@ -580,11 +599,11 @@ k_dropout_grad(T *dsrc, const R *grad, float *dbias, uint64_t rows, uint64_t col
     /* column j of the block's tx * 8: its rows y = 0, 1, .. in order */
     for (unsigned j = threadIdx.x; j < tx * 8; j += kThreads) {
         if (c0 + j < cols) {
-            float s = 0.f;
+            double s = 0;
             for (unsigned q = 0; q < ty; q++) {
-                s += lds[q * tx * 8 + j];
+                s += (double)lds[q * tx * 8 + j];
             }
-            dbias[(uint64_t)blockIdx.y * cols + c0 + j] = s;
+            dbias[(uint64_t)blockIdx.y * cols + c0 + j] = (float)s;
         }
     }
 }
@@ -1725,6 +1744,7 @@ struct GradPlan {
     unsigned tx;                 /* lanes side by side */
     unsigned parts;
     uint64_t blocks_x;
+    bool     deep;               /* a lane has more than kFewRows rows */
 };
 
 GradPlan grad_plan(uint64_t rows, uint64_t cols)
@@ -1745,6 +1765,7 @@ GradPlan grad_plan(uint64_t rows, uint64_t cols)
     const uint64_t most = div_up(rows, ty * 4);
     parts   = parts < most ? parts : most;
     g.parts = parts > 0 ? (unsigned)parts : 1;
+    g.deep  = div_up(rows, g.parts * ty) > kFewRows;
     return g;
 }
 
@@ -2075,12 +2096,21 @@ ucs_status_t ucg_builtin_dev_sum_dropout_grad(ucg_builtin_dev_ctx_t *ctx,
         const GradPlan plan = grad_plan(rows, cols);
         float *out          = plan.parts > 1 ? static_cast<float*>(workspace) : dbias;
         const dim3 grid((unsigned)plan.blocks_x, plan.parts);
+        const auto launch = [&](auto aligned, auto deep) {
+            hipLaunchKernelGGL((k_dropout_grad<R, T, decltype(aligned)::value, decltype(deep)::value>),
+                               grid, dim3(kThreads), 0, stream, d, g, out, rows, cols, plan.tx, rng);
+        };
+        const auto launch_deep = [&](auto aligned) {
+            if (plan.deep) {
+                launch(aligned, std::true_type());
+            } else {
+                launch(aligned, std::false_type());
+            }
+        };
         if (cols % 8 == 0 && rng.offset % 8 == 0) {
-            hipLaunchKernelGGL((k_dropout_grad<R, T, true>), grid, dim3(kThreads), 0, stream, d,
-                               g, out, rows, cols, plan.tx, rng);
+            launch_deep(std::true_type());
         } else {
-            hipLaunchKernelGGL((k_dropout_grad<R, T, false>), grid, dim3(kThreads), 0, stream, d,
-                               g, out, rows, cols, plan.tx, rng);
+            launch_deep(std::false_type());
         }
         if (plan.parts > 1) {
             hipLaunchKernelGGL(k_join_bias, dim3((unsigned)div_up(cols, 16)), dim3(kThreads), 0,
