@@ -96,3 +96,31 @@ def test_bias_gradient_of_many_rows(dev_ctx, dt, rows, cols, offset):
     want = head + (rows - head) * 2.0 ** -24
     assert np.abs(db.get() - want).max() <= 33 * U * want
     assert (d.get() == g).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt,experts", [("bfloat16", 512), ("float16", 256), ("float32", 256), ("bfloat16", 60)])
+def test_balance_sums_of_many_rows(dev_ctx, dt, experts):
+    """Blocks that begin with rows whose probability for expert 0 is 1, and
+    whose log sum exp is 16, and go on with rows of which a sum in 32 bits would
+    lose both values whole. At most 32 rows are added up in 32 bits, then six
+    steps over lanes, one over waves, a part's and the last rounding: 41 u. A
+    probability of 1 is exact, of 1 - 2^-24 to 2 u; the others weigh nothing."""
+    tokens = (1 << 27) // max(experts, 64)           # 64 rows and more to a lane
+    low, z = 16.7, 0.0035                            # exp(-low) = 0.94 * 2^-24, z^2 = 0.8 * 256 * 2^-24
+    kinds = np.full((2, experts), -np.inf)
+    kinds[0, 0], kinds[1, 0], kinds[1, 1] = 16.0, z - low, z
+    kinds = R.to_storage(kinds, dt)
+    head = np.arange(tokens) % (tokens // 256) < 16 * 64 // min(64, max(1, experts * 2 // 16))
+    p, lse = R.softmax(R.from_storage(kinds, dt))
+    la = Arr(dev_ctx, kinds[np.where(head, 0, 1)])
+    ia = Arr(dev_ctx, np.zeros((tokens, 1), np.int32))
+    c, s = Arr(dev_ctx, np.zeros(experts + 1, np.int64)), Arr(dev_ctx, np.zeros(experts + 1, np.float32))
+    ws = dev_ctx.alloc(max(16, dev_ctx.balance_workspace(tokens, experts)))
+    dev_ctx.balance(dt, la.ptr, ia.ptr, tokens, experts, 1, c.ptr, s.ptr, index_dt="int32", workspace=ws)
+    dev_ctx.sync()
+    n = np.array([head.sum(), (~head).sum()], np.float64)
+    got = s.get().astype(np.float64)
+    want = np.append(n @ p, n @ lse ** 2)
+    assert (np.abs(got - want) <= 43 * U * want).all()
+    assert c.get()[0] == tokens == c.get()[-1]
