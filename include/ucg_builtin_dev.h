@@ -383,11 +383,12 @@ ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
  *   d = logp - old (rounded to 32 bits), r = exp(d), q = ref - logp
  *   cut: A > 0 and d > log(1 + clip_high), or A < 0 and d < log(1 - clip_low)
  *        (both limits rounded to 32 bits)
- *   pg = -A * (cut ? 1 + clip_high or 1 - clip_low : r)
+ *   pg = -A * (cut ? 1 + clip_high or 1 - clip_low : r), 0 for A = 0
  *   kl = exp(q) - q - 1 (0 without ref)
  *   loss = mean of pg + kl_coef * mean of kl
  *
- * where the mean is over the group's tokens, or, with per_sequence, over the
+ * r and pg are held in 32 bits: an r that is not cut and passes their range is
+ * infinite. The mean is over the group's tokens, or, with per_sequence, over the
  * group's rows that have a token, of each row's mean. sums (FLOAT32, 2 values:
  * the sums of pg and of kl, of the rows' means with per_sequence) and counts
  * (INT64, 3 values: tokens, rows that have one, cut tokens) add up over the

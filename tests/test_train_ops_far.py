@@ -124,3 +124,31 @@ def test_balance_sums_of_many_rows(dev_ctx, dt, experts):
     want = np.append(n @ p, n @ lse ** 2)
     assert (np.abs(got - want) <= 43 * U * want).all()
     assert c.get()[0] == tokens == c.get()[-1]
+
+
+# ---- values at the ends of their range -----------------------------------------------
+@gpu
+@pytest.mark.parametrize("per_row", [False, True])
+def test_policy_without_advantage(dev_ctx, per_row):
+    """A = 0 (of either sign) gives 0 for any ratio, also one that is infinite
+    in 32 bits, and cuts nothing; a NaN stays one."""
+    d = np.array([0.5, 87, 89, 200, 1e30, np.inf, -5, -200, -np.inf, 88.72, 1, 2, 3], np.float32)
+    for sign in (0.0, -0.0):
+        la, oa = Arr(dev_ctx, d[None]), Arr(dev_ctx, np.zeros((1, len(d)), np.float32))
+        aa = Arr(dev_ctx, np.full(1 if per_row else (1, len(d)), sign, np.float32))
+        s, c, g = Arr(dev_ctx, np.ones(2, np.float32)), Arr(dev_ctx, np.ones(3, np.int64)), Arr(dev_ctx, d[None])
+        ws = dev_ctx.alloc(dev_ctx.policy_workspace(1, len(d)))
+
+        def run():
+            dev_ctx.policy("float32", la.ptr, oa.ptr, aa.ptr, 1, len(d), s.ptr, c.ptr, adv_per_row=per_row,
+                           workspace=ws)
+            dev_ctx.policy_grad("float32", g.ptr, la.ptr, oa.ptr, aa.ptr, 1, len(d), c.ptr, adv_per_row=per_row)
+            dev_ctx.sync()
+        run()
+        assert s.get().tolist() == [0, 0] and c.get().tolist() == [len(d), 1, 0]
+        assert (g.get() == 0).all()
+        x = d[None].copy()
+        x[0, 3] = np.nan
+        la = Arr(dev_ctx, x)
+        run()
+        assert np.isnan(s.get()[0]) and (np.isnan(g.get()[0]) == np.isnan(x[0])).all()

@@ -1143,6 +1143,8 @@ __device__ __forceinline__ float exp_series(float q)
     return __builtin_fmaf(s, q, 0.5f);
 }
 
+constexpr float kExpEnd = 88.f;        /* its exponential is finite */
+
 /* exp(q) - q - 1; both forms are computed: no branch around either */
 __device__ __forceinline__ float exp_less(float q)
 {
@@ -1161,17 +1163,21 @@ __device__ __forceinline__ float exp_minus(float q)
 }
 
 /* What an advantage makes of its tokens: d with A's sign is compared with
- * `limit` (a token is cut goes by d itself, not by its rounded exponential;
- * A = 0 has no limit), and `cap` is the ratio of a cut token. */
+ * `limit` (a token is cut goes by d itself, not by its rounded exponential),
+ * `cap` is the ratio of a cut token and `count` what it adds to the counts.
+ * A = 0 cuts none; its limit keeps ratios that are infinite in 32 bits from
+ * its product, which is 0 for any d. */
 struct Advantage {
-    float a, limit, cap;
+    float    a, limit, cap;
+    unsigned count;
 
     __device__ __forceinline__ Advantage() = default;
     __device__ __forceinline__ Advantage(float x, const Policy &p)
     {
-        a     = x;
-        limit = x > 0.f ? p.up : x < 0.f ? -p.down : INFINITY;
+        a     = x + 0.f;              /* -0 as 0 */
+        limit = x > 0.f ? p.up : x < 0.f ? -p.down : kExpEnd;
         cap   = x > 0.f ? p.ratio_up : p.ratio_down;
+        count = x > 0.f || x < 0.f ? 0x10000u : 0u;
     }
     __device__ __forceinline__ bool cuts(float d) const
     {
@@ -1298,7 +1304,7 @@ struct PolicyAcc {
             r = (is ? w.cap : r) * -w.a;
             vpg += on ? r : 0.f;
             n += on;
-            n += (on & is) ? 0x10000u : 0u;
+            n += (on & is) ? w.count : 0u;
             if constexpr (REF) {
                 float e = exp_less((float)t.ref[k] - x);
                 asm("" : "+v"(e));
