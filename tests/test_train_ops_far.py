@@ -12,6 +12,33 @@ from test_train_ops import DTS, U, Arr, balance_bounds, gpu, ptr
 from xucg_amd import group as G
 
 
+# ---- refusals (CPU) --------------------------------------------------------------------
+def test_freed_buffers_are_refused():
+    """A buffer that was freed has the address NULL, which for an operand that may
+    be left out would mean that: the call would run without bias or mask."""
+    ctx = xucg_amd.DevContext.__new__(xucg_amd.DevContext)   # no GPU is needed to refuse
+    ctx.handle, ctx.device = None, 0
+    for kind in (xucg_amd.DevBuffer, xucg_amd.HostBuffer):
+        gone = kind.__new__(kind)
+        gone.ptr, gone.nbytes = None, 1 << 20
+        at = [k << 20 for k in range(1, 9)]
+        for what, call in (
+                ("bias", lambda: ctx.sum_dropout("float32", at[0], at[1:2], 4, 8, 0.1, 1, bias=gone)),
+                ("residual", lambda: ctx.sum_dropout("float32", at[0], at[1:2], 4, 8, 0.1, 1, residual=gone)),
+                ("rng", lambda: ctx.sum_dropout("float32", at[0], at[1:2], 4, 8, 0.1, 1, rng=gone)),
+                ("dbias", lambda: ctx.sum_dropout_grad("float32", at[0], at[1], 4, 8, 0.1, 1, dbias=gone)),
+                ("mask", lambda: ctx.balance("float32", at[0], at[1], 4, 8, 2, at[2], at[3], mask=gone)),
+                ("base", lambda: ctx.balance_grad("float32", at[0], at[1], 4, 8, 2, at[2], base=gone)),
+                ("ref", lambda: ctx.policy("float32", *at[:3], 4, 8, *at[3:5], ref=gone, workspace=at[5])),
+                ("grad_loss", lambda: ctx.policy_grad("float32", *at[:4], 4, 8, at[4], grad_loss=gone)),
+                ("workspace", lambda: ctx.policy("float32", *at[:3], 4, 8, *at[3:5], workspace=gone))):
+            with pytest.raises(ValueError, match=f"{what}: the buffer is freed"):
+                call()
+    for what in (np.zeros(64, np.uint8), "ws"):
+        with pytest.raises(TypeError, match="workspace: device memory wanted"):
+            ctx.policy("float32", *at[:3], 4, 8, *at[3:5], workspace=what)
+
+
 # ---- members without work ------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dt", DTS)

@@ -260,6 +260,8 @@ class DevContext:
         except AttributeError:
             if not isinstance(x, (DevBuffer, HostBuffer)):
                 raise TypeError(f"{name}: device memory wanted, got {type(x)}") from None
+            if not x.ptr:             # NULL is an operand left out
+                raise ValueError(f"{name}: the buffer is freed")
             span = n if step == row or not n else (n // row - 1) * step + row
             if span * DTYPE_SIZE[_DT[dt]] > x.nbytes:
                 raise ValueError(f"{name}: a buffer of {span} {dt} wanted, got {x.nbytes} bytes")
@@ -329,6 +331,10 @@ class DevContext:
             if workspace.get_device() != self.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace: a contiguous tensor on cuda:{self.device} wanted")
             return workspace.data_ptr(), workspace.nbytes
+        if not isinstance(workspace, (DevBuffer, HostBuffer)):
+            raise TypeError(f"workspace: device memory wanted, got {type(workspace)}")
+        if not workspace.ptr:
+            raise ValueError("workspace: the buffer is freed")
         return workspace.ptr, workspace.nbytes
 
     @staticmethod
