@@ -6,6 +6,7 @@ operations that a value goes through (u = 2^-24 for each in fp32)."""
 import numpy as np
 import pytest
 
+import test_train_ops as near
 import xucg_amd
 from oracle import train_ref as R
 from test_train_ops import DTS, U, Arr, balance_bounds, gpu, ptr
@@ -179,3 +180,159 @@ def test_policy_without_advantage(dev_ctx, per_row):
         la = Arr(dev_ctx, x)
         run()
         assert np.isnan(s.get()[0]) and (np.isnan(g.get()[0]) == np.isnan(x[0])).all()
+
+
+# ---- loops past their first pass -----------------------------------------------------
+# The sizes are the smallest that make each kernel's loops repeat: the rows of
+# the bias' gradient (256 parts of 4 lanes, four rows a pass: 4096), the rows of
+# the balance gradient (1024 blocks), the rows and the parts of the policy join
+# (64 blocks; 8 parts to each of 64 lanes), the parts of the policy kernels.
+@gpu
+@pytest.mark.parametrize("dt,grad_dt", [("float32", "float32"), ("bfloat16", "bfloat16"),
+                                        ("float16", "float16"), ("bfloat16", "float32"),
+                                        ("float16", "float32")])
+@pytest.mark.parametrize("rows,cols,offset", [(4101, 512, 0), (4101, 515, 5)])
+def test_bias_gradient_of_several_passes(dev_ctx, dt, grad_dt, rows, cols, offset):
+    near.test_sum_dropout_grad(dev_ctx, dt, grad_dt, rows, cols, offset)
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("tokens,experts,topk", [(5000, 1000, 4), (17000, 256, 8)])
+def test_balance_of_several_passes(dev_ctx, dt, tokens, experts, topk):
+    near.test_balance(dev_ctx, dt, tokens, experts, topk)
+
+
+@gpu
+@pytest.mark.parametrize("dt,rows,cols", [(dt, *s) for dt in DTS for s in ((20000, 5), (1, 600000))] +
+                         [("float32", 1, 5000001), ("bfloat16", 2, 4300005)])
+def test_policy_of_several_passes(dev_ctx, dt, rows, cols):
+    near.test_policy(dev_ctx, dt, rows, cols)
+
+
+@gpu
+def test_policy_of_very_many_rows(dev_ctx):
+    """More rows than a grid has at once (2^20 blocks of 256), one token each, all
+    of ratio 1: the sums are the advantages', whole numbers."""
+    rows = (1 << 28) + 300
+    adv = np.ones(rows, np.float32)
+    adv[-300:] = 3
+    want = -(1 << 28) - 900.0
+    x, a = dev_ctx.alloc(2 * rows), dev_ctx.alloc(4 * rows)
+    a.upload(adv)
+    chunk = np.zeros(1 << 26, np.uint16)
+    for at in range(0, 2 * rows, chunk.nbytes):
+        x.upload(chunk[:(2 * rows - at) // 2], at)
+    d, ws = dev_ctx.alloc(2 * rows), dev_ctx.alloc(dev_ctx.policy_workspace(rows, 1))
+    s, c = Arr(dev_ctx, np.ones(2, np.float32)), Arr(dev_ctx, np.ones(3, np.int64))
+    kw = dict(adv_per_row=True)
+    dev_ctx.policy("bfloat16", x, x, a, rows, 1, s.ptr, c.ptr, workspace=ws, **kw)
+    dev_ctx.policy_grad("bfloat16", d, x, x, a, rows, 1, c.ptr, **kw)
+    dev_ctx.sync()
+    assert s.get().tolist() == [np.float32(want), 0] and c.get().tolist() == [rows, rows, 0]
+    got = d.download(np.uint16, rows)
+    one, three = R.to_storage(np.array([-1.0, -3.0]) / rows, "bfloat16")
+    assert (got[:1 << 28] == one).all() and (got[1 << 28:] == three).all()
+    for b in (x, a, d, ws):
+        b.free()
+
+
+# ---- gradients in place --------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("rows,cols,offset", [(5, 13, 3), (4101, 512, 8), (4101, 515, 5), (1 << 18, 65, 1)])
+def test_dropout_gradient_in_place(dev_ctx, dt, rows, cols, offset):
+    """dsrc = grad: the bits of the call that is not in place."""
+    rng = np.random.default_rng(cols)
+    g = R.to_storage(rng.normal(size=(rows, cols)).astype(np.float32), dt)
+    for with_bias in (True, False):
+        got = []
+        for in_place in (False, True):
+            ga, db = Arr(dev_ctx, g), Arr(dev_ctx, np.ones(cols, np.float32))
+            d = ga if in_place else Arr(dev_ctx, g * 0)
+            ws = dev_ctx.alloc(max(16, dev_ctx.sum_dropout_grad_workspace(rows, cols)))
+            dev_ctx.sum_dropout_grad(dt, d.ptr, ga.ptr, rows, cols, 0.3, 7, offset=offset,
+                                     dbias=db.ptr if with_bias else None, workspace=ws)
+            dev_ctx.sync()
+            got.append((d.get(), db.get()))
+        assert (got[0][0] == got[1][0]).all() and (got[0][1] == got[1][1]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("tokens,experts", [(9, 5), (5000, 1000), (17000, 256), (70000, 8), (30011, 60)])
+def test_balance_gradient_in_place(dev_ctx, dt, tokens, experts):
+    """dlogits = logits and dlogits = base, also while the next rows are on the
+    way: the bits of the call that is not in place."""
+    rng = np.random.default_rng(tokens)
+    x, base = (R.to_storage(rng.normal(size=(tokens, experts)).astype(np.float32) * s, dt) for s in (2, 1e-3))
+    mask = (rng.random(tokens) < 0.8).astype(np.uint8)
+    counts = np.append(rng.integers(0, tokens, experts), max(1, mask.sum())).astype(np.int64)
+    ca, ma = Arr(dev_ctx, counts), Arr(dev_ctx, mask)
+    got = {}
+    for where in ("apart", "logits", "base", "apart, no base", "logits, no base"):
+        la, ba = Arr(dev_ctx, x), Arr(dev_ctx, base)
+        d = {"l": la, "b": ba}.get(where[0]) or Arr(dev_ctx, x * 0)
+        dev_ctx.balance_grad(dt, d.ptr, la.ptr, tokens, experts, 2, ca.ptr, mask=ma.ptr, balance_coef=0.5,
+                             z_coef=0.1, base=None if "no base" in where else ba.ptr)
+        dev_ctx.sync()
+        got[where] = d.get()
+        assert where[0] == "l" or (la.get() == x).all()
+        assert where[0] == "b" or (ba.get() == base).all()
+    assert (got["logits"] == got["apart"]).all() and (got["base"] == got["apart"]).all()
+    assert (got["logits, no base"] == got["apart, no base"]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("rows,cols", [(3, 7), (300, 33), (20000, 5), (9, 4100), (1, 600000)])
+def test_policy_gradient_in_place(dev_ctx, dt, rows, cols):
+    """dlogp = logp, old or ref: the bits of the call that is not in place."""
+    rng = np.random.default_rng(cols)
+    old = -rng.random((rows, cols)).astype(np.float32) * 3
+    arrays = [R.to_storage(a, dt) for a in (old + rng.normal(size=old.shape).astype(np.float32) * 0.3, old,
+                                            old + rng.normal(size=old.shape).astype(np.float32) * 0.3)]
+    adv = Arr(dev_ctx, rng.normal(size=old.shape).astype(np.float32))
+    mask = (rng.random(old.shape) < 0.7).astype(np.uint8)
+    ma, ca = Arr(dev_ctx, mask), Arr(dev_ctx, np.array([mask.sum() + 1, rows, 0], np.int64))
+    got = {}
+    for where in (None, 0, 1, 2):
+        a = [Arr(dev_ctx, v) for v in arrays]
+        d = Arr(dev_ctx, arrays[0] * 0) if where is None else a[where]
+        dev_ctx.policy_grad(dt, d.ptr, a[0].ptr, a[1].ptr, adv.ptr, rows, cols, ca.ptr, ref=a[2].ptr, mask=ma.ptr,
+                            kl_coef=0.3)
+        dev_ctx.sync()
+        got[where] = d.get()
+        for i in range(3):
+            assert i == where or (a[i].get() == arrays[i]).all()
+    assert all((got[w] == got[None]).all() for w in got)
+
+
+# ---- sums near their bound -----------------------------------------------------------
+def sums_tolerance(x, mask, ws):
+    """What the balance sums may be off: a probability's and a log sum exp's own
+    error, 32 rows of a lane, six steps over lanes, one over waves, a part's and
+    the last rounding - whatever the number of tokens."""
+    rel, dl = balance_bounds(x, mask)
+    e, n = x.shape[1], len(x) if mask is None else int((mask != 0).sum())
+    z = 2 * dl * np.sqrt(n * ws[e]) + n * dl * dl
+    return np.append((rel + 41 * U) * ws[:e], z + 41 * U * ws[e])
+
+
+@gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("tokens,experts,topk", [(40000, 8, 2), (33000, 5, 1), (20000, 16, 2)])
+def test_balance_sums_miss_no_token(dev_ctx, dt, tokens, experts, topk):
+    """The bound is tight enough to see a token of tens of thousands: without
+    any one of some, the oracle's own sums are past it."""
+    rng = np.random.default_rng(experts)
+    x, index, mask = near.balance_inputs(rng, dt, tokens, experts, topk, np.int64, "some")
+    _, _, c, s, _ = near.run_balance(dev_ctx, dt, x, index, mask)
+    wc, ws = R.balance_stats(x, index, mask)
+    tol = sums_tolerance(x, mask, ws)
+    assert (c.get() == wc).all()
+    off = np.abs(s.get().astype(np.float64) - ws)
+    assert (off <= tol).all(), (off / tol).max()
+    p, lse = R.softmax(x)
+    for t in np.flatnonzero(mask)[:50]:
+        assert (np.append(p[t], lse[t] ** 2) > 2 * tol).any()
