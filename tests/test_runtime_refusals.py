@@ -28,3 +28,23 @@ def test_refused_peer_import_names_its_cause():
     assert codes == [1, 1]
     for out in outs:
         assert "import of the peer's descriptor (open, 2097152 bytes; descriptors are taken by " in out
+
+
+@pytest.mark.gpu
+def test_a_refused_call_is_reported_once(dev_ctx):
+    """A HIP call that fails is the error of the call that made it, and not of
+    the launches after it, which ask the runtime for the last error."""
+    import numpy as np
+    from xucg_amd import _lib
+    host = np.zeros(1 << 16, np.uint8)               # was never registered
+    x = dev_ctx.alloc(4096)
+    x.upload(np.ones(1024, np.float32))
+    counts, sums, loss = dev_ctx.alloc(72), dev_ctx.alloc(36), dev_ctx.alloc(12)
+    for launch in (lambda: dev_ctx.reduce_checked("sum", "float32", x.ptr, x.ptr, 1024),
+                   lambda: dev_ctx.balance("float32", x, x, 0, 8, 1, counts, sums),
+                   lambda: dev_ctx.sum_dropout("float32", x, [x], 1, 1024, 0.0, 1),
+                   lambda: dev_ctx.balance_loss(counts, sums, 8, 1, loss)):
+        assert _lib.dev().ucg_builtin_dev_host_unregister(dev_ctx.handle, host.ctypes.data) != 0
+        launch()
+    dev_ctx.sync()
+    assert (x.download(np.float32, 1024) == 2).all()

@@ -45,6 +45,9 @@ ucs_status_t hip_status(hipError_t e, const char *what)
     if (e == hipSuccess) {
         return UCS_OK;
     }
+    /* it is reported here: left with the runtime it would be reported again, by
+     * whatever asks after its next launch */
+    (void)hipGetLastError();
     ucs_status_t st;
     switch (e) {
     case hipErrorNoDevice:
