@@ -273,7 +273,10 @@ ucs_status_t ucg_builtin_dev_reduce_tree(ucg_builtin_dev_ctx_t *ctx, ucg_dev_op_
  * once, or captured graphs that may replay at once, need one each). No
  * reference counterpart (the reference combines, it does not train).
  * FLOAT32, BFLOAT16 and FLOAT16 only; arithmetic in 32 bits or more, rounded
- * once. Zero rows, columns or tokens are allowed unless stated otherwise. */
+ * once. Zero rows, columns or tokens are allowed unless stated otherwise: the
+ * sums, counts and losses of a member without work are zeros. Operands
+ * that lie in one another are refused unless named as allowed; an operand with
+ * a row step counts from its first element to its last, steps included. */
 
 /* dst = residual + dropout(sum of srcs + bias), rows x cols, contiguous.
  *
@@ -387,13 +390,14 @@ ucs_status_t ucg_builtin_dev_balance_grad(ucg_builtin_dev_ctx_t *ctx,
  *   kl = exp(q) - q - 1 (0 without ref)
  *   loss = mean of pg + kl_coef * mean of kl
  *
- * r and pg are held in 32 bits: an r that is not cut and passes their range is
- * infinite. The mean is over the group's tokens, or, with per_sequence, over the
- * group's rows that have a token, of each row's mean. sums (FLOAT32, 2 values:
- * the sums of pg and of kl, of the rows' means with per_sequence) and counts
- * (INT64, 3 values: tokens, rows that have one, cut tokens) add up over the
- * members of a group. Masked tokens are not looked at, whatever they hold:
- * their gradient is 0. Without a token the loss is 0. */
+ * r and pg are held in 32 bits: r is off by up to (1.25 |d| + 2) 2^-24 of
+ * itself, and one that is not cut and passes their range is infinite. The mean
+ * is over the group's tokens, or, with per_sequence, over the group's rows that
+ * have a token, of each row's mean. sums (FLOAT32, 2 values: the sums of pg and
+ * of kl, of the rows' means with per_sequence) and counts (INT64, 3 values:
+ * tokens, rows that have one, cut tokens) add up over the members of a group.
+ * Masked tokens are not looked at, whatever they hold: their gradient is 0.
+ * Without a token the loss is 0. */
 typedef struct ucg_builtin_dev_policy_params {
     int    dt;            /* ucg_dev_dtype_t of logp, old, ref and dlogp */
     int    adv_per_row;   /* adv holds rows values, else rows x cols */

@@ -182,6 +182,21 @@ def test_policy_without_advantage(dev_ctx, per_row):
         assert np.isnan(s.get()[0]) and (np.isnan(g.get()[0]) == np.isnan(x[0])).all()
 
 
+@gpu
+def test_policy_ratio_is_as_near_as_documented(dev_ctx):
+    """The gradient of A = -1 over one token is the ratio itself (clip_low = 1
+    cuts none): off by (1.25 |d| + 2) u, for d = 0 not at all."""
+    d = np.append(np.linspace(-80, 80, 4001), [0.0, 1e-30, 88.0, -87.0]).astype(np.float32)[None]
+    la, oa = Arr(dev_ctx, d), Arr(dev_ctx, d * 0)
+    aa, g, c = Arr(dev_ctx, -np.ones(1, np.float32)), Arr(dev_ctx, d * 0), Arr(dev_ctx, np.ones(3, np.int64))
+    dev_ctx.policy_grad("float32", g.ptr, la.ptr, oa.ptr, aa.ptr, 1, d.size, c.ptr, adv_per_row=True, clip_low=1.0)
+    dev_ctx.sync()
+    d64 = d.astype(np.float64)
+    off = np.abs(g.get() / np.exp(d64) - 1) / U
+    assert (off <= 1.25 * np.abs(d64) + 2).all()
+    assert (g.get()[d == 0] == 1).all()
+
+
 # ---- loops past their first pass -----------------------------------------------------
 # The sizes are the smallest that make each kernel's loops repeat: the rows of
 # the bias' gradient (256 parts of 4 lanes, four rows a pass: 4096), the rows of

@@ -3,8 +3,9 @@
  * (ucg_builtin_dev.h): the sum of several operands with dropout in its
  * epilogue, a router's balance loss and the clipped policy loss, each with its
  * gradient. All of them stream their operands from HBM once; sums are held in
- * fp32 over a few rows and joined in fp64 in an order that depends on the
- * sizes alone, so a call gives the same bits every time (no float atomics).
+ * fp32 over at most 32 rows of a lane (one vector in the policy terms) and
+ * joined in fp64 in an order that depends on the sizes alone, so a call gives
+ * the same bits every time (no float atomics).
  */
 #include <hip/hip_runtime.h>
 
@@ -313,10 +314,15 @@ constexpr int kWaveElems = 512;
  *
  * HBM bounds it: 16384 x 8192 bf16 with an fp32 residual takes 206 us = 6.5 TB/s
  * (this library's plain copy reaches 6.8), four bf16 sources of 4096 x 4096 33.4
- * us = 6.0 TB/s; without the numbers (p = 0) it takes as long. Waves whose parts
- * begin inside a line share it with their neighbours: `map` deals them to the
- * XCDs in runs (8191 x 4097 bf16 46.3 against 48.3 us; on lines the identity is
- * faster, 16384 x 8192 bf16 132 against 149 us).
+ * us = 6.0 TB/s; without the numbers (p = 0) it takes as long. Fan-ins without
+ * an instantiation of their own load their second source on behind the numbers
+ * and lose nothing by it (4096 x 4096 bf16: 7 sources 49.1 us = 6.1 TB/s, 8 55.7,
+ * 12 77.5, 15 95.6 us). Waves whose parts begin inside a line share it with their
+ * neighbours: `map` deals them to the XCDs in runs (8191 x 4097 bf16 43.3 against
+ * 46.5 us; on lines the identity is faster, 16384 x 8192 bf16 126.0 against 127.9
+ * us). They stay behind calls on lines (8192 x 4096 34.3 us) although HBM reads
+ * only 2 % and writes 4 % more than there: each access of a wave touches a line
+ * more, and the lines at its ends are written in two pieces.
  *
  * `inv` is 2^64 / cols rounded up (unused for one column): the quotient by
  * cols is its high product, or one less (the rounding adds i * e / 2^64 < 1
@@ -475,7 +481,7 @@ k_sum_dropout(R *dst, SrcList srcs, unsigned nsrc, const T *bias, const R *resid
  * rounded to 32 (half the join's bytes: 8192 x 4096 bf16 27.7 us, 28.1 in 64),
  * parts are joined in 64.
  *
- * 8192 x 4096 bf16 takes 25.2 us = 5.3 TB/s, and 4.7 for the join of 128 parts
+ * 8192 x 4096 bf16 takes 24.6 us = 5.5 TB/s, and 4.8 for the join of 128 parts
  * (less than half of a launch is its bytes); fp32 54 us with it = 5.0 TB/s. With
  * rows in chunks of neighbours instead of dealt to the parts fp32 took 63, with
  * the eight fp32 columns side by side 74 us. 8191 x 4097 bf16 takes 41 us: twice
@@ -767,9 +773,9 @@ constexpr int kBalanceThreads = 1024;  /* 16 waves: one block to a CU */
  * 32 bits, all else in 64; a block's part is rounded to 32, as the sums are that
  * the group adds up, and the loss is taken from those.
  *
- * 65536 x 256 bf16, top 8: 11.7 us, and 4.7 with the loss for the join. Without the
- * softmax 8.6: the exponentials and sums of 16 M probabilities do not hide behind
- * 38 MB here, and 256 blocks start and end together. 512 of them take longer for
+ * 65536 x 256 bf16, top 8: 13.3 us, and 4.8 with the loss for the join. Without the
+ * softmax 3.9 less: the exponentials and sums of 16 M probabilities do not hide
+ * behind 38 MB here, and 256 blocks start and end together. 512 of them take longer for
  * the join than they save (18.1 against 17.3 us in all). */
 template <typename T, typename I, int G, int NV, bool EVEN, bool DEEP>
 __global__ void __launch_bounds__(kBalanceThreads)
@@ -957,9 +963,10 @@ k_balance_loss(const int64_t *counts, const float *sums, Balance p, float *loss)
  * N topk / experts. It is the middle one of three, so that one expert that is
  * much liked does not set it (their mean, summed in 64 bits over the block, took
  * 0.7 us, in fp32 over a row's lanes 0.2 to 0.5).
- * 49999 x 160 bf16 with a base takes 11.8 us = 4.1 TB/s: a row lies in 32 lanes of
- * which 20 have columns, and a block goes over its rows three or four times (1536
- * and 2048 blocks, and one row in flight, took longer). */
+ * 49999 x 160 bf16 with a base takes 11.8 us a pass = 4.1 TB/s: the exchanges of
+ * each row (a maximum and two sums, five steps each over 32 lanes, of which this
+ * layout gives columns to 20) wait for one another, and a wave has two rows in
+ * flight beside them (1536 and 2048 blocks, and one row in flight, took longer). */
 template <typename T, int G, int NV, bool EVEN>
 __global__ void __launch_bounds__(kThreads)
 k_balance_grad(const T *logits, const uint8_t *mask, const int64_t *counts, const T *base,
@@ -1118,7 +1125,13 @@ struct PolicySum {
     }
 };
 
-/* by the hardware's base-2 exponential (1 ulp); the scaling rounds off |x| u */
+/* By the hardware's base-2 exponential (1 ulp), of the rounded product: (1.25 |x|
+ * + 2) u of the result, u = 2^-24. A ratio between 1/e and e is off by 3.3 u at
+ * most, one of e^20 by 27 u. The product in two parts (2 u for any x) is a choice
+ * not made: four to six instructions more for each exponential took 0.1-0.3 us of
+ * 27 on 1024 x 8192 fp32 terms, 1.0 of 25.4 on their gradient and 1.9 of 21.3 on
+ * 512 x 16384 bf16 terms, for digits of ratios that the clip replaces or that
+ * carry no weight. */
 __device__ __forceinline__ float exp_of(float x)
 {
     return __builtin_amdgcn_exp2f(x * kLog2e);
@@ -1400,14 +1413,16 @@ __device__ __forceinline__ void policy_write(const PolicySum &s, const Policy &p
     }
 }
 
-/* 1024 x 8192 fp32 with a reference takes 20 us = 5.4 TB/s and 6 for the join of
- * 8192 parts: 37 vector instructions a token, two exponentials among them, leave
+/* 1024 x 8192 fp32 with a reference takes 20.7 us = 5.3 TB/s and 6.4 for the join
+ * of 8192 parts: 37 vector instructions a token, two exponentials among them, leave
  * HBM about the bound. Twice the tokens in flight took 29.2 us in all against
  * 27.5, half of them as long as these.
  *
  * A wave does one part of 64 / lanes rows at a time: `steps` vectors of each
- * of the lanes that share the row, all in flight at once. NT = kSingle: the
- * only block, which has the parts in LDS and joins them too. */
+ * of the lanes that share the row, all in flight at once. The tokens behind the
+ * last whole vector are one lane's, one after the other: 2048 rows of 1023 bf16
+ * take 14.3 us in all where 1024 take 11.9, of 7 9.4 where 8 take 8.0. NT =
+ * kSingle: the only block, which has the parts in LDS and joins them too. */
 constexpr int kSingle      = 512;
 constexpr int kSingleParts = 1024;
 
@@ -1523,7 +1538,8 @@ __device__ __forceinline__ void policy_slope(const Tokens<T, V> &t, const Advant
 }
 
 /* 513 x 12345 bf16 with a reference and advantages by tokens takes 15.9 us = 5.2
- * TB/s, 1024 x 8192 fp32 25.5 us = 5.6 TB/s. */
+ * TB/s, 1024 x 8192 fp32 25.5 us = 5.6 TB/s. A row's last tokens as in k_policy:
+ * 2048 x 1023 bf16 9.6 us, 1024 6.6. */
 template <typename T, bool REF, bool ROW, bool LINES>
 __global__ void __launch_bounds__(kThreads)
 k_policy_grad(PolicyIn<T, REF, ROW, LINES> in, const int32_t *row_tokens, const int64_t *counts,
