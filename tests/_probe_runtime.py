@@ -51,16 +51,17 @@ def exporter(sock):
 def importer(sock):
     hip = runtime()
     buf = (ctypes.c_char * (1 << 20))()
-    st = hip.hipSetDevice(0)
-    reg = st or hip.hipHostRegister(buf, ctypes.c_size_t(len(buf)), ctypes.c_uint(0))
-    if reg == 0:
-        hip.hipHostUnregister(buf)
-    hip.hipGetLastError()
     msg, fds, _, _ = socket.recv_fds(sock, 64, 1)
-    peer, by_value = json.loads(msg)
-    peer = peer or st or take(hip, (ctypes.c_int * 4)(), fds[0], by_value)
+    st, by_value = json.loads(msg)
+    answers = {}
+    if hip.hipSetDevice(0) == 0:          # without a device nothing is known
+        answers["host_register"] = hip.hipHostRegister(buf, ctypes.c_size_t(len(buf)), ctypes.c_uint(0))
+        if answers["host_register"] == 0:
+            hip.hipHostUnregister(buf)
+        if st == 0:                       # the exporter has it, and could import it itself
+            answers["peer_import"] = take(hip, (ctypes.c_int * 4)(), fds[0], by_value)
     sock.send(b"y")
-    return {"peer_import": peer, "host_register": reg}
+    return answers
 
 
 def main():
